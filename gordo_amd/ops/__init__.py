@@ -51,3 +51,19 @@ def is_available() -> bool:
     if not torch.cuda.is_available():
         return False
     return _load_extension() is not None
+
+
+from .checkpoint8 import Saved8, linear8, load8, save8, weight_grad8  # noqa: E402
+from .recurrence import gated_scan, gated_step  # noqa: E402
+
+__all__ = [
+    "ext",
+    "is_available",
+    "gated_scan",
+    "gated_step",
+    "Saved8",
+    "save8",
+    "load8",
+    "linear8",
+    "weight_grad8",
+]

@@ -128,3 +128,24 @@ void lstm_bwd_h32_launch(torch::Tensor dh_out, torch::Tensor gates_seq,
 void lstm_dw_h32_launch(torch::Tensor dgates, torch::Tensor x_seq, torch::Tensor h_seq,
                         torch::Tensor partial, torch::Tensor db_partial,
                         int64_t BT, int64_t T);
+
+void gated_scan_fwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Tensor> h0,
+                           c10::optional<torch::Tensor> lengths, torch::Tensor y, torch::Tensor h_last,
+                           c10::optional<torch::Tensor> states, c10::optional<torch::Tensor> codes,
+                           c10::optional<torch::Tensor> scales);
+
+void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Tensor> lengths,
+                           torch::Tensor states, c10::optional<torch::Tensor> codes,
+                           c10::optional<torch::Tensor> scales, torch::Tensor dy,
+                           c10::optional<torch::Tensor> dh_last, torch::Tensor dp,
+                           c10::optional<torch::Tensor> dh0);
+
+void gated_step_launch(torch::Tensor p, int64_t dim, torch::Tensor state, c10::optional<torch::Tensor> slots,
+                       torch::Tensor out, torch::Tensor y);
+
+void save8_launch(torch::Tensor x, torch::Tensor codes, torch::Tensor scales);
+
+void load8_launch(torch::Tensor codes, torch::Tensor scales, torch::Tensor x);
+
+void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor scales, torch::Tensor dw,
+                         c10::optional<torch::Tensor> db);

@@ -22,6 +22,8 @@ try:
         "gordo_amd/ops/hip/lstm_h32_kernels.hip",
         "gordo_amd/ops/hip/lstm_wide_kernels.hip",
         "gordo_amd/ops/hip/lstm_wide256_kernels.hip",
+        "gordo_amd/ops/hip/gated_scan_kernels.hip",
+        "gordo_amd/ops/hip/checkpoint8_kernels.hip",
     ]
     hip_sources = [s for s in hip_sources if os.path.exists(s)]
     if hip_sources and torch.version.hip is not None:
@@ -31,7 +33,10 @@ try:
                 sources=hip_sources,
                 extra_compile_args={
                     "cxx": ["-O3", "-std=c++17"],
-                    "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+                    # without packed fp32: some forms that the compiler makes
+                    # of ordinary float code have given wrong results on gfx950
+                    "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
                 },
             )
         )

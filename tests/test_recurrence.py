@@ -1,0 +1,431 @@
+"""Gated linear recurrence (ops.recurrence) against its definition in 64 bits.
+
+Tolerances: an output of type t is off by its rounding, eps(t)/2 of the value,
+and by the 32-bit arithmetic before it. A gate's relative error is at most
+2^-20 (exp and reciprocal of an argument below 16 in magnitude); one token adds
+that much of k (x - h) and two roundings of h, and errors are never amplified
+(f <= 1), so after T tokens a state is off by at most 2^-20 M + T 2^-22 M, M
+being the largest magnitude that takes part. The gradient's recursion is the
+same one; its products of three to five such factors are allowed four times that.
+"""
+import pytest
+import torch
+
+from gordo_amd.ops import gated_scan, gated_step
+
+EVERY = 16
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(0)
+
+
+# ------------------------------------------------------------------ definition
+def kept8(v):
+    """[..., D] in float64 as 8-bit codes keep it."""
+    out = torch.empty_like(v)
+    for at in range(0, v.shape[-1], 32):
+        w = v[..., at : at + 32]
+        _, e = torch.frexp(w.abs().amax(-1, keepdim=True))
+        step = torch.exp2((e - 7).clamp_min(-126).double())
+        out[..., at : at + 32] = torch.clamp(torch.round(w / step), -127, 127) * step
+    return out
+
+
+def definition(p, dim, h0, lengths, dy, dh, keep="input"):
+    """(y, h_last, dp, dh0) in float64 on the CPU, token by token."""
+    p, dy, dh = (t.detach().cpu().double() for t in (p, dy, dh))
+    B, T, width = p.shape
+    h0 = torch.zeros(B, dim, dtype=torch.float64) if h0 is None else h0.detach().cpu().double()
+    n = [T] * B if lengths is None else [min(max(int(v), 0), T) for v in lengths.cpu()]
+    y = torch.zeros(B, T, dim, dtype=torch.float64)
+    dp = torch.zeros_like(p)
+    last, dh0 = h0.clone(), dh.clone()
+    for b in range(B):
+        h, states = h0[b], []
+        for t in range(n[b]):
+            states.append(h)
+            x, r = p[b, t, :dim], p[b, t, dim : 2 * dim]
+            f = torch.sigmoid(r)
+            h = f * h + (1 - f) * x
+            y[b, t] = h
+            if width == 3 * dim:
+                z = p[b, t, 2 * dim :]
+                y[b, t] = h * z * torch.sigmoid(z)
+        last[b] = h
+        q = p[b]
+        if keep == "int8":
+            q = torch.cat([kept8(part) for part in p[b].split(dim, -1)], -1)
+            for t in range(n[b]):
+                if t % EVERY:
+                    f = torch.sigmoid(q[t - 1, dim : 2 * dim])
+                    states[t] = f * states[t - 1] + (1 - f) * q[t - 1, :dim]
+        c = dh[b]
+        for t in range(n[b] - 1, -1, -1):
+            x, f = q[t, :dim], torch.sigmoid(q[t, dim : 2 * dim])
+            g = dy[b, t]
+            if width == 3 * dim:
+                z = q[t, 2 * dim :]
+                s = torch.sigmoid(z)
+                h = f * states[t] + (1 - f) * x
+                dp[b, t, 2 * dim :] = g * h * (s + z * s * (1 - s))
+                g = g * z * s
+            g = g + c
+            dp[b, t, :dim] = g * (1 - f)
+            dp[b, t, dim : 2 * dim] = g * (states[t] - x) * f * (1 - f)
+            c = g * f
+        dh0[b] = c
+    return y, last, dp, dh0
+
+
+def inputs(B, T, D, dtype, device, gate=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    parts = 3 if gate else 2
+    p = torch.randn(B, T, parts, D, generator=g)
+    p[:, :, 1] = p[:, :, 1] * 1.5 + 1
+    p = p.reshape(B, T, parts * D).to(dtype)
+    h0, dh = torch.randn(B, D, generator=g), torch.randn(B, D, generator=g)
+    dy = torch.randn(B, T, D, generator=g).to(dtype)
+    return [t.to(device) for t in (p, h0, dy, dh)]
+
+
+def near(got, want, scale, T, what, wide=1.0):
+    got, want = got.detach().cpu(), want
+    assert got.shape == want.shape, what
+    eps = torch.finfo(got.dtype).eps
+    allowed = eps / 2 * want.abs() * 1.0001 + wide * scale * (2.0**-20 + T * 2.0**-22)
+    if got.dtype == torch.float16:
+        allowed = allowed + 2.0**-25  # half a step of the subnormal numbers
+    off = (got.double() - want).abs() - allowed
+    assert torch.isfinite(got).all(), what
+    assert off.max() <= 0 if off.numel() else True, (what, float(off.max()))
+
+
+def check(p, D, h0, lengths, dy, dh, keep="input"):
+    p = p.detach().requires_grad_()
+    h = None if h0 is None else h0.detach().requires_grad_()
+    y, last = gated_scan(p, D, h, lengths, keep=keep)
+    leaves = (p,) if h is None else (p, h)
+    grads = torch.autograd.grad((y, last), leaves, (dy, dh))
+    want = definition(p, D, h0, lengths, dy, dh, keep)
+    assert y.dtype == p.dtype and last.dtype == torch.float32
+    T = p.shape[1]
+    m = max(1.0, *(float(t.abs().max()) for t in (want[1], p.detach().double().cpu().nan_to_num(0)) if t.numel()))
+    mg = max(1.0, *(float(t.abs().max()) for t in want[2:] if t.numel()))
+    near(y, want[0], m * m, T, "y")
+    near(last, want[1], m, T, "h_last")
+    near(grads[0], want[2], 4 * m * m * mg, T, "dp")
+    if h is not None:
+        near(grads[1], want[3], mg, T, "dh0")
+    return y, last, grads
+
+
+# ----------------------------------------------------------------------- the scan
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "plain"])
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (3, 15, 2), (2, 16, 33), (2, 17, 64), (5, 49, 25), (1, 144, 50), (2, 129, 130)])
+def test_scan_and_gradient(device, dtype, gate, keep, B, T, D):
+    p, h0, dy, dh = inputs(B, T, D, dtype, device, gate)
+    check(p, D, h0, None, dy, dh, keep)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize("D", [7, 40])
+def test_lengths_leave_padding_alone(device, keep, index, D):
+    """Empty and full sequences, lengths outside the range, and padding that holds NaN and infinities."""
+    T = 37
+    p, h0, dy, dh = inputs(8, T, D, torch.bfloat16, device)
+    lengths = torch.tensor([0, 1, 15, 16, 17, T, T + 100, -3], dtype=index)
+    for b, n in enumerate([0, 1, 15, 16, 17, T, T, 0]):
+        p[b, n:, ::2] = float("nan")
+        p[b, n:, 1::2] = float("-inf")
+        dy[b, n:] = float("inf")
+    y, last, (dp, dh0) = check(p, D, h0, lengths.to(device), dy, dh, keep)
+    assert not y[0].any() and not dp[0].any() and not y[2, 15:].any() and not dp[2, 15:].any()
+    assert torch.equal(last[0], h0[0]) and torch.equal(last[7], h0[7]) and torch.equal(dh0[0], dh[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_padding_of_zeros_is_a_longer_batch(device, dtype):
+    p, h0, dy, dh = inputs(3, 40, 10, dtype, device)
+    lengths = torch.full((3,), 25, device=device)
+    y, last = gated_scan(p, 10, h0, lengths)
+    short, short_last = gated_scan(p[:, :25].contiguous(), 10, h0)
+    assert torch.equal(y[:, :25], short) and torch.equal(last, short_last)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("first,extra", [(0, 6), (4, 4), (1, 5), (3, 8)])
+def test_strides(device, first, extra):
+    """A slice of a wider buffer, at even and odd places, time and batch swapped."""
+    B, T, D = 3, 35, 12
+    p, h0, dy, dh = inputs(B, T, D, torch.bfloat16, device)
+    wide = torch.full((T, B, first + 3 * D + extra), 9.0, dtype=p.dtype, device=device)
+    view = wide[:, :, first : first + 3 * D].transpose(0, 1)
+    view.copy_(p)
+    dyw = torch.full((B, T, D + extra), 9.0, dtype=p.dtype, device=device)[..., extra:]
+    dyw.copy_(dy)
+    a = check(view, D, h0, None, dyw, dh)
+    b = check(p, D, h0, None, dy, dh)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2][0], b[2][0])
+    turned = p.transpose(1, 2).contiguous().transpose(1, 2)  # last axis not of unit stride
+    assert torch.equal(gated_scan(turned, D, h0)[0], b[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_parts_of_the_gradient(device):
+    """Only y, only h_last, an expanded gradient, a projection alone, no h0."""
+    B, T, D = 2, 33, 6
+    p, h0, dy, dh = inputs(B, T, D, torch.float32, device)
+    check(p, D, None, None, dy, dh)
+    check(p, D, h0, None, torch.ones((), device=device).expand(B, T, D), torch.zeros_like(dh))
+    q = p.clone().requires_grad_()
+    only_last = torch.autograd.grad(gated_scan(q, D, h0)[1].sum(), q)[0]
+    want = definition(p, D, h0, None, torch.zeros_like(dy), torch.ones_like(dh))[2]
+    near(only_last, want, 40.0, T, "dp of h_last")
+    h = h0.clone().requires_grad_()
+    dh0 = torch.autograd.grad(gated_scan(p, D, h)[0].sum(), h)[0]
+    want = definition(p, D, h0, None, torch.ones_like(dy), torch.zeros_like(dh))[3]
+    near(dh0, want, 40.0, T, "dh0 of y")
+
+
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("gate", [True, False])
+def test_definition_against_differences(gate, keep):
+    """The formula of the gradient is the derivative of the formula of the scan
+    (with codes: where nothing is lost, that is at values that codes hold)."""
+    B, T, D = 2, 5, 3
+    p, h0, dy, dh = inputs(B, T, D, torch.float32, "cpu", gate)
+    p = kept8(p.double().reshape(B, T, -1, D)).reshape(B, T, -1)
+    y, last, dp, dh0 = definition(p, D, h0, None, dy, dh, keep)
+    loss = lambda p, h: sum(float((a * b.double()).sum()) for a, b in zip(definition(p, D, h, None, dy, dh)[:2], (dy, dh)))  # noqa: E731
+    step = 1e-5  # central differences: error step^2 and 1e-16 / step
+    g = torch.Generator().manual_seed(3)
+    for _ in range(6):
+        v, w = torch.randn(p.shape, generator=g, dtype=torch.float64), torch.randn(h0.shape, generator=g, dtype=torch.float64)
+        slope = (loss(p + step * v, h0.double() + step * w) - loss(p - step * v, h0.double() - step * w)) / (2 * step)
+        assert abs(slope - float((dp * v).sum() + (dh0 * w).sum())) < 1e-7 * max(1.0, abs(slope))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_long_memory_keeps_its_digits(device):
+    """k = 2^-20: 1 - k has five bits of it in 32 bits, the scan all of them."""
+    r = 13.862942695617676  # log(2^20 - 1)
+    T, D = 512, 4
+    p = torch.zeros(1, T, 2 * D, device=device)
+    p[..., :D], p[..., D:] = 1.0, r
+    y, last = gated_scan(p, D)
+    k = torch.sigmoid(-torch.tensor(r, dtype=torch.float64))
+    want = 1 - (1 - k) ** T  # h after T tokens of x = 1
+    # a gate is off by 2^-20 of itself, each of T updates rounds h, which is below 2^-10
+    assert (last.double().cpu() - want).abs().max() < 2.0**-20 * want + T * 2.0**-35
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_extreme_gates(device):
+    """Gates that are wide open or shut pass or hold the state exactly."""
+    p = torch.zeros(1, 40, 6, device=device)
+    p[..., :2] = torch.arange(40.0, device=device)[:, None]
+    p[..., 2], p[..., 3] = 200.0, -200.0
+    p[..., 4:] = 1.0
+    h0 = torch.tensor([[5.0, 7.0]], device=device)
+    y, last = gated_scan(p[..., :4].contiguous(), 2, h0)
+    assert (y[..., 0] == 5).all() and torch.equal(y[0, :, 1].cpu(), torch.arange(40.0))
+    p[..., 2], p[..., 3] = float("inf"), float("-inf")
+    y, last = gated_scan(p[..., :4].contiguous(), 2, h0)
+    assert (y[..., 0] == 5).all() and torch.equal(y[0, :, 1].cpu(), torch.arange(40.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty(device):
+    h0 = torch.randn(2, 3, device=device)
+    y, last = gated_scan(torch.randn(2, 0, 9, device=device), 3, h0)
+    assert y.shape == (2, 0, 3) and torch.equal(last, h0)
+    y, last = gated_scan(torch.randn(0, 4, 6, device=device), 3)
+    assert y.shape == (0, 4, 3) and last.shape == (0, 3)
+
+
+def test_scan_refuses():
+    p = torch.randn(2, 4, 9)
+    for bad in (
+        lambda: gated_scan(p.double(), 3),
+        lambda: gated_scan(p.to(torch.int32), 3),
+        lambda: gated_scan(p[0], 3),
+        lambda: gated_scan(p, 4),
+        lambda: gated_scan(p, 9),
+        lambda: gated_scan(p, 0),
+        lambda: gated_scan(p, 3.0),
+        lambda: gated_scan(p, 3, torch.randn(2, 3).double()),
+        lambda: gated_scan(p, 3, torch.randn(3, 2)),
+        lambda: gated_scan(p, 3, torch.randn(1, 3)),
+        lambda: gated_scan(p, 3, lengths=torch.tensor([1.0, 2.0])),
+        lambda: gated_scan(p, 3, lengths=torch.tensor([1])),
+        lambda: gated_scan(p, 3, lengths=[1, 2]),
+        lambda: gated_scan(p, 3, h0=torch.randn(2, 3, device="meta")),
+        lambda: gated_scan(p, 3, keep="fp8"),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ----------------------------------------------------------------------- the step
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "plain"])
+@pytest.mark.parametrize("B,D", [(1, 1), (3, 50), (2, 255), (4, 1030)])
+def test_steps_are_the_scan(device, dtype, gate, B, D):
+    """Token by token, the step gives what the scan gives, and the scan's state goes on in it."""
+    T = 5
+    p, h0, dy, dh = inputs(B, T, D, dtype, device, gate)
+    want = definition(p, D, h0, None, dy, dh)
+    state = h0.clone()
+    for t in range(T):
+        y = gated_step(p[:, t], state)
+        near(y, want[0][:, t], 25.0, T, "y")
+    near(state, want[1], 5.0, T, "state")
+    state = gated_scan(p[:, :3], D, h0)[1]
+    gated_step(p[:, 3], state)
+    near(gated_step(p[:, 4], state), want[0][:, 4], 25.0, T, "y after a scan")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize("apart", [False, True], ids=["in place", "out"])
+def test_slots(device, index, apart):
+    """Padding rows, slots that come again, and slots that no row names."""
+    S, D = 9, 70
+    slots = torch.tensor([4, -1, 7, 4, 2, S, 4, -(2**31), 7, 2**31 - 1], dtype=index)
+    p, _, _, _ = inputs(len(slots), 1, D, torch.float32, device)
+    p = p[:, 0]
+    before = torch.randn(S, D, generator=torch.Generator().manual_seed(1)).to(device)
+    state = before.clone()
+    out = torch.full_like(state, 3.0) if apart else None
+    y = gated_step(p, state, slots.to(device), out=out)
+    want = before.cpu().double()
+    for b, s in enumerate(slots.tolist()):
+        if not 0 <= s < S:
+            assert not y[b].any()
+            continue
+        x, r, z = p[b].cpu().double().split(D)
+        f = torch.sigmoid(r)
+        want[s] = f * want[s] + (1 - f) * x
+        near(y[b], want[s] * z * torch.sigmoid(z), 25.0, 3, f"y of row {b}")
+    named = torch.tensor(sorted({s for s in slots.tolist() if 0 <= s < S}))
+    rest = torch.tensor([s for s in range(S) if s not in named.tolist()])
+    got = state if out is None else out
+    near(got.cpu()[named], want[named], 5.0, 3, "states")
+    assert torch.equal(state.cpu()[rest], before.cpu()[rest])
+    if apart:
+        assert (out.cpu()[rest] == 3.0).all() and torch.equal(state, before)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_of_nothing(device):
+    state = torch.randn(3, 4, device=device)
+    assert gated_step(torch.randn(0, 8, device=device), state, torch.zeros(0, dtype=torch.int32, device=device)).shape == (0, 4)
+    none = torch.empty(0, 4, device=device)
+    assert not gated_step(torch.randn(2, 8, device=device), none, torch.zeros(2, dtype=torch.int64, device=device)).any()
+
+
+def test_step_refuses():
+    p, state = torch.randn(2, 9), torch.randn(5, 3)
+    slots = torch.tensor([0, 1])
+    big = torch.randn(11, 3)
+    for bad in (
+        lambda: gated_step(p.double(), state, slots),
+        lambda: gated_step(p[:, :8], state, slots),
+        lambda: gated_step(p[None], state, slots),
+        lambda: gated_step(p, state.half(), slots),
+        lambda: gated_step(p, state.t().contiguous().t(), slots),
+        lambda: gated_step(p, state[0], slots),
+        lambda: gated_step(p, state),
+        lambda: gated_step(p, state, slots.float()),
+        lambda: gated_step(p, state, slots[:1]),
+        lambda: gated_step(p, state, torch.zeros(2, dtype=torch.int32, device="meta")),
+        lambda: gated_step(p, state, slots, out=torch.randn(4, 3)),
+        lambda: gated_step(p, state, slots, out=state.half()),
+        lambda: gated_step(p, big[:5], slots, out=big[1:6]),
+        lambda: gated_step(p.requires_grad_(), state, slots),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ------------------------------------------------------------- on the GPU alone
+@pytest.mark.gpu
+def test_same_inputs_same_bits():
+    p, h0, dy, dh = inputs(2, 700, 96, torch.bfloat16, "cuda")
+    lengths = torch.tensor([700, 433], device="cuda")
+    runs = [check(p, 96, h0, lengths, dy, dh, "int8") for _ in range(3)]
+    for y, last, (dp, dh0) in runs[1:]:
+        assert torch.equal(y, runs[0][0]) and torch.equal(last, runs[0][1])
+        assert torch.equal(dp, runs[0][2][0]) and torch.equal(dh0, runs[0][2][1])
+
+
+@pytest.mark.gpu
+def test_on_a_stream_of_its_own():
+    p, h0, dy, dh = inputs(2, 100, 40, torch.float32, "cuda")
+    want = check(p, 40, h0, None, dy, dh)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = check(p, 40, h0, None, dy, dh)
+    s.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2][0], want[2][0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [30, 900, 6000])
+def test_captured(T):
+    """Forward, backward and step in a graph, replayed with eager work between."""
+    D = 32
+    p, h0, dy, dh = inputs(1, T, D, torch.bfloat16, "cuda")
+    row, state = p[:, 0].clone(), h0.clone()
+
+    def work(p, h0, dy, dh, row, state):
+        p, h0 = p.detach().requires_grad_(), h0.detach().requires_grad_()
+        y, last = gated_scan(p, D, h0, keep="int8")
+        dp, dh0 = torch.autograd.grad((y, last), (p, h0), (dy, dh))
+        with torch.no_grad():
+            return y.detach(), last.detach(), dp, dh0, gated_step(row, state)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        work(p, h0, dy, dh, row, state.clone())
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(p, h0, dy, dh, row, state)
+    for seed in range(1, 4):
+        fresh = inputs(1, T, D, torch.bfloat16, "cuda", seed=seed)
+        for a, b in zip((p, h0, dy, dh, row, state), (*fresh, fresh[0][:, 0], fresh[1])):
+            a.copy_(b)
+        eager_state = state.clone()
+        want = work(p.clone(), h0, dy, dh, row, eager_state)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*out, state), (*want, eager_state)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Two sequences more than 2^31 elements apart, tokens far apart too."""
+    T, D = 20, 16
+    p, h0, dy, dh = inputs(2, T, D, torch.bfloat16, "cuda")
+    far = 2**31 + 64
+    buf = torch.empty(far + (T - 1) * 2**20 + 3 * D, dtype=torch.bfloat16, device="cuda")
+    view = buf.as_strided((2, T, 3 * D), (far, 2**20, 1))
+    view.copy_(p)
+    a, b = check(view, D, h0, None, dy, dh), check(p, D, h0, None, dy, dh)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2][0], b[2][0])
