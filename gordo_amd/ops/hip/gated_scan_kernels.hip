@@ -26,11 +26,49 @@ __device__ __forceinline__ float gs_rcp(float x) { return __builtin_amdgcn_rcpf(
 // exp overflows to +inf for x far below 0, whose reciprocal is the right 0
 __device__ __forceinline__ float gs_sigmoid(float x) { return gs_rcp(1.f + __expf(-x)); }
 
-// V neighbouring elements of type E
+// V neighbouring elements of type E as the register that a load fills. They stay
+// packed until they are used: 16-bit pairs as 32-bit floats would take twice the
+// registers, and how many tokens a wave holds is what decides the speed here.
 template <class E, int V>
-struct alignas(sizeof(typename E::store) * V) GsVec {
-    typename E::store v[V];
+struct GsPack {
+    typedef typename E::store store;
+    static_assert(sizeof(store) * V <= 4, "a register");
+    unsigned int w;
+    __device__ __forceinline__ void load(const store* from) {
+        if constexpr (sizeof(store) * V == 2) w = *(const unsigned short*)from;
+        else w = *(const unsigned int*)from;
+    }
+    __device__ __forceinline__ float get(int v) const {
+        if constexpr (sizeof(store) == 4) return __uint_as_float(w);
+        else if constexpr (std::is_same<E, C8Bf16>::value) return __uint_as_float(v == 0 ? w << 16 : w & 0xffff0000u);
+        else return E::up((unsigned short)(v == 0 ? w : w >> 16));
+    }
+    // what was unpacked before this is not kept for what comes after
+    __device__ __forceinline__ void pin() { asm("" : "+v"(w)); }
+    static __device__ __forceinline__ void put(store* to, const float (&f)[V]) {
+        if constexpr (V == 1) to[0] = E::down(f[0]);
+        else *(unsigned int*)to = pair(f[0], f[1]);
+    }
+    static __device__ __forceinline__ unsigned int pair(float a, float b) {
+        return (unsigned int)E::down(a) | ((unsigned int)E::down(b) << 16);
+    }
 };
+
+// Where waves share a CU by registers, a scheduler that interleaves many tokens to
+// hide latencies spills: two tokens at a time are enough beside the other waves.
+template <int W>
+__device__ __forceinline__ void gs_fence(int i) {
+    if (W > 1 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+}
+
+// f(integral_constant 0 .. N-1): for where an instruction wants a constant
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void gs_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        gs_for<N, I + 1>(f);
+    }
+}
 
 struct GsArgs {
     const void* p;          // [B][T][P*D], rows at sb, st
@@ -51,6 +89,12 @@ struct GsArgs {
     float* dh0;             // [B][D] or null
     int B, T, D, Dp;
     int tps;                // lanes of one sequence
+    int nJ;                 // blocks' tiles along T
+    int groups;             // 64-lane groups of channels
+    // chained blocks (null: a block walks all its tiles)
+    unsigned int* ticket;
+    unsigned long long* agg;  // [nJ][groups][V][64]: a tile's (A, H), all ones until it is there
+    unsigned int* prefix;     // [nJ / GS_LB][groups][V][64]: state after a run of GS_LB tiles
 };
 
 __device__ __forceinline__ int gs_len(const GsArgs& a, int b) {
@@ -73,94 +117,312 @@ __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
     l.live = b < a.B && l.d < a.D;
     l.b = b < a.B ? (int)b : a.B - 1;   // lanes without a channel read one that exists
     l.d = l.d < a.D ? l.d : a.D - V;
-    l.len = l.live ? gs_len(a, l.b) : 0;
+    l.len = l.live ? gs_len(a, l.b) : a.T;
     return l;
+}
+
+// ---------------------------------------------------------------------------
+// Blocks of W waves take W tiles side by side in time. A tile maps the state
+// before it to the state after it by h -> A h + H; the waves put their (A, H)
+// into LDS, and each folds those before it, in their order.
+//
+// With few channels, time is split over blocks too. Block j needs the state
+// after tile j - 1, and gets it without a second pass over the data: every block
+// publishes its (A, H) as soon as it has it, and every GS_LB-th block, which
+// folds the GS_LB - 1 before it, the state after itself. So a block reads at most
+// GS_LB words a channel, the serial chain has nJ / GS_LB links, and the order of
+// the folds is fixed: the same inputs give the same bits.
+//
+// (A, H) is one 64-bit word, the prefix one 32-bit word: a word is there when it
+// is no longer all ones (a NaN is published as the canonical one), so data and
+// flag arrive together and no fence is needed; accesses are at agent scope, since
+// the blocks of a chain run on XCDs with L2 caches of their own. Blocks take their
+// place in the chain from a ticket, so each waits only for blocks that run
+// already: every wait ends. The bound on the spins is there so that a broken
+// workspace gives NaN and no hang.
+// ---------------------------------------------------------------------------
+#define GS_LB 16
+#define GS_SPINS (1 << 20)
+
+__device__ __forceinline__ unsigned int gs_word(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
+
+__device__ __forceinline__ void gs_publish(unsigned long long* to, float2 m) {
+    __hip_atomic_store(to, ((unsigned long long)gs_word(m.y) << 32) | gs_word(m.x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ float2 gs_then(float2 first, float2 second) {
+    return float2{first.x * second.x, fmaf(second.x, first.y, second.y)};
+}
+
+template <int V, int W>
+struct GsChain {
+    float2 part[2][W][V][64];
+    float2 pred[W > 1 ? GS_LB : 1][V][64];
+    float start[V][64];
+    unsigned int ticket;
+};
+
+// A block's place: its group of channels, its tile, counted in the order of the
+// chain, and the first tile that it does not do.
+template <int V, int W>
+__device__ __forceinline__ void gs_place(const GsArgs& a, GsChain<V, W>& s, int& cg, int& j, int& end) {
+    cg = blockIdx.x;
+    j = 0;
+    end = a.nJ;
+    if constexpr (W > 1) {
+        if (a.ticket != nullptr) {
+            if (threadIdx.x == 0) s.ticket = atomicAdd(a.ticket, 1u) + 1u;  // it starts at all ones
+            __syncthreads();
+            const unsigned int t = s.ticket;
+            j = (int)(t / (unsigned int)a.groups);
+            cg = (int)(t - (unsigned int)j * a.groups);
+            end = j + 1;
+        }
+    }
+}
+
+// The state that enters this wave's tile, from `carry` (the state that enters the
+// block's first tile; of the chain's first block where blocks are chained), and in
+// `carry` the state after the block's last tile. `mine`: this wave's map; `order`:
+// this wave's place in the block, 0 first. j counts tiles in the chain's order.
+template <int V, int W>
+__device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int cg, int j, int order, int lane,
+                                        const float2 (&mine)[V], float (&carry)[V], float (&in)[V]) {
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) in[v] = carry[v];
+        return;
+    }
+    const int par = j & 1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s.part[par][order][v][lane] = mine[v];
+    __syncthreads();
+    if (a.ticket != nullptr) {
+        const int i = j % GS_LB, g = j / GS_LB;
+        const bool more = j + 1 < a.nJ;
+        if (order == W - 1 && i < GS_LB - 1 && more) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float2 m = s.part[par][0][v][lane];
+#pragma unroll 2
+                for (int w = 1; w < W; ++w) m = gs_then(m, s.part[par][w][v][lane]);
+                gs_publish(a.agg + (((int64_t)j * a.groups + cg) * V + v) * 64 + lane, m);
+            }
+        }
+        // the wave's share of the blocks before: all loads go out, then all are looked at
+        const int Q = (GS_LB + W - 1) / W;
+        unsigned long long word[Q][V];
+        unsigned int first[V];
+        const bool chained = order == 0 && g > 0;
+        bool there;
+        int spins = 0;
+        do {
+            there = true;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (q * W + order < i)
+                        word[q][v] = __hip_atomic_load(a.agg + (((int64_t)(g * GS_LB + q * W + order) * a.groups + cg) * V + v) * 64 + lane,
+                                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (chained) {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    first[v] = __hip_atomic_load(a.prefix + (((int64_t)(g - 1) * a.groups + cg) * V + v) * 64 + lane,
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (q * W + order < i) there &= (unsigned int)word[q][v] != ~0u;
+            if (chained) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) there &= first[v] != ~0u;
+            }
+        } while (!__all(there) && ++spins < GS_SPINS);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                if (q * W + order < i)
+                    s.pred[q * W + order][v][lane] = float2{__uint_as_float((unsigned int)word[q][v]),
+                                                            __uint_as_float((unsigned int)(word[q][v] >> 32))};
+            if (order == 0) s.start[v][lane] = chained ? __uint_as_float(first[v]) : carry[v];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float h = s.start[v][lane];
+#pragma unroll 2
+            for (int q = 0; q < i; ++q) {
+                const float2 m = s.pred[q][v][lane];
+                h = fmaf(m.x, h, m.y);
+            }
+            carry[v] = h;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float h = carry[v];
+#pragma unroll 2
+        for (int w = 0; w < W; ++w) {
+            if (w == order) in[v] = h;
+            const float2 m = s.part[par][w][v][lane];
+            h = fmaf(m.x, h, m.y);
+        }
+        carry[v] = h;
+    }
+    if (a.ticket != nullptr && order == W - 1 && j % GS_LB == GS_LB - 1 && j + 1 < a.nJ) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            __hip_atomic_store(a.prefix + (((int64_t)(j / GS_LB) * a.groups + cg) * V + v) * 64 + lane, gs_word(carry[v]),
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+// all ones: no word of the chain is there yet, and the next ticket is 0
+__global__ __launch_bounds__(256) void gs_clear(uint4* to, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = uint4{~0u, ~0u, ~0u, ~0u};
 }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-template <class E, int V, int P, bool KEEP>
-__global__ __launch_bounds__(64) void gs_fwd(GsArgs a) {
-    typedef GsVec<E, V> vec;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 64 + lane;
+
+// The codes and scales of a tile of one part. The 32 values of a group are pairs
+// in 16 lanes (V = 2) or one in each of 32 (V = 1); a tile has 16 tokens, so
+// lane i of 16 collects the scale of token i and stores it once.
+template <class E, int V>
+__device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&raw)[GS_R], bool live, bool mine, int64_t row,
+                                          int64_t step, int left, int dd, int lane) {
+    unsigned int scale = 0;
+    signed char* to = a.codes + row * a.Dp + dd;
+#pragma unroll
+    for (int i = 0; i < GS_R; ++i) {
+        float f[V];
+        unsigned int top = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            f[v] = live ? raw[i].get(v) : 0.f;
+            top = max(top, c8_mag(f[v]));
+        }
+        top = c8_max16(top);
+        if constexpr (V == 1) top = max(top, (unsigned int)__shfl_xor((int)top, 16, 64));
+        const unsigned int s = c8_scale(top);
+        const float inv = c8_inv(s);
+        scale = (lane & 15) == i ? s : scale;
+        if (mine && i < left) {
+            if constexpr (V == 2) *(short*)to = (short)((c8_code(f[0], inv) & 0xff) | (c8_code(f[1], inv) << 8));
+            else to[0] = (signed char)c8_code(f[0], inv);
+        }
+        to += step * a.Dp;
+        __builtin_amdgcn_sched_barrier(0);  // one token after the other: interleaved, they need too many registers
+    }
+    const int i = lane & 15;
+    if (mine && i < left && (V == 2 || (lane & 16) == 0))
+        a.scales[(row + i * step) * (a.Dp / C8_GROUP) + dd / C8_GROUP] = (unsigned char)scale;
+}
+
+template <class E, int V, int P, bool KEEP, int W>
+__global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(GsArgs a) {
+    typedef GsPack<E, V> pack;
+    __shared__ GsChain<V, W> chain;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    int cg, j, end;
+    gs_place<V, W>(a, chain, cg, j, end);
+    const int64_t id = (int64_t)cg * 64 + lane;
     const GsLane l = gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
     typename E::store* y = (typename E::store*)a.y + (int64_t)l.b * a.T * a.D + l.d;
 
-    float h[V];
+    float carry[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = a.h0 != nullptr ? a.h0[(int64_t)l.b * a.D + l.d + v] : 0.f;
+    for (int v = 0; v < V; ++v) carry[v] = a.h0 != nullptr ? a.h0[(int64_t)l.b * a.D + l.d + v] : 0.f;
 
-    for (int tile = 0; tile < nT; ++tile) {
-        const int t0 = tile * GS_R;
-        if (a.states != nullptr && l.live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
-        }
-        vec raw[P][GS_R];
+    for (; j < end; ++j) {
+        const int tile = j * W + wid, t0 = tile * GS_R;
+        pack raw[P][GS_R];
 #pragma unroll
         for (int i = 0; i < GS_R; ++i) {
             const int t = min(t0 + i, a.T - 1);
 #pragma unroll
-            for (int q = 0; q < P; ++q) raw[q][i] = *(const vec*)(p + (int64_t)t * a.st + q * a.D);
+            for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
+        }
+        float k[GS_R][V], h[V];
+        float2 m[V];
+        const bool whole = __all(l.len >= t0 + GS_R);  // every token of the tile is one of every lane's sequence
+        auto gates = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
+#pragma unroll
+            for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) {
+                const bool in = FULL || t0 + i < l.len;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                    if constexpr (W > 1) {
+                        const float x = raw[0][i].get(v);
+                        // selected, not multiplied by 0: padding may hold anything
+                        m[v].y = in ? fmaf(k[i][v], x - m[v].y, m[v].y) : m[v].y;
+                        m[v].x = in ? fmaf(-k[i][v], m[v].x, m[v].x) : m[v].x;
+                    }
+                }
+                gs_fence<W>(i);
+            }
+        };
+        if (whole) gates(std::true_type{});
+        else gates(std::false_type{});
+        gs_join<V, W>(a, chain, cg, j, wid, lane, m, carry, h);
+        if (a.states != nullptr && l.live && tile < nT) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
         }
         if constexpr (KEEP) {
-            const int64_t ng = a.Dp / C8_GROUP;
-            const bool mine = id < (int64_t)a.B * a.tps;
+            const int64_t row = ((int64_t)l.b * a.T + t0) * P;
             const int dd = (int)(id % a.tps) * V;  // channel, padding included
 #pragma unroll
             for (int q = 0; q < P; ++q) {
 #pragma unroll
-                for (int i = 0; i < GS_R; ++i) {
-                    float f[V];
-                    unsigned int top = 0;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        f[v] = l.live ? E::up(raw[q][i].v[v]) : 0.f;
-                        top = max(top, c8_mag(f[v]));
-                    }
-                    top = c8_max16(top);
-                    if constexpr (V == 1) top = max(top, (unsigned int)__shfl_xor((int)top, 16, 64));
-                    const unsigned int s = c8_scale(top);
-                    const float inv = c8_inv(s);
-                    if (mine && t0 + i < a.T) {
-                        const int64_t row = ((int64_t)l.b * a.T + t0 + i) * P + q;
-                        signed char* c = a.codes + row * a.Dp + dd;
-                        if constexpr (V == 2) {
-                            *(short*)c = (short)((c8_code(f[0], inv) & 0xff) | (c8_code(f[1], inv) << 8));
-                        } else {
-                            c[0] = (signed char)c8_code(f[0], inv);
-                        }
-                        if ((dd & (C8_GROUP - 1)) == 0) a.scales[row * ng + dd / C8_GROUP] = (unsigned char)s;
-                    }
-                }
+                for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
+                gs_encode<E, V>(a, raw[q], l.live, id < (int64_t)a.B * a.tps, row + q, P, a.T - t0, dd, lane);
             }
         }
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
-            const bool in = t0 + i < l.len;
-            vec out;
+        for (int i = 0; i < GS_R; ++i) raw[0][i].pin();
+        auto run = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float k = gs_sigmoid(-E::up(raw[1][i].v[v])), x = E::up(raw[0][i].v[v]);
-                // selected, not multiplied by 0: padding may hold anything
-                h[v] = in ? fmaf(k, x - h[v], h[v]) : h[v];
-                float o = h[v];
-                if constexpr (P == 3) {
-                    const float z = E::up(raw[2][i].v[v]);
-                    o *= z * gs_sigmoid(z);
+            for (int i = 0; i < GS_R; ++i) {
+                const bool in = FULL || t0 + i < l.len;
+                float out[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
+                    out[v] = h[v];
+                    if constexpr (P == 3) {
+                        const float z = raw[2][i].get(v);
+                        out[v] *= z * gs_sigmoid(z);
+                    }
+                    out[v] = in ? out[v] : 0.f;
                 }
-                out.v[v] = E::down(in ? o : 0.f);
+                if (l.live && (FULL || t0 + i < a.T)) pack::put(y + (int64_t)(t0 + i) * a.D, out);
+                gs_fence<W>(i);
             }
-            if (l.live && t0 + i < a.T) *(vec*)(y + (int64_t)(t0 + i) * a.D) = out;
-        }
-    }
-    if (l.live) {
+        };
+        if (whole) run(std::true_type{});
+        else run(std::false_type{});
+        // from the wave that has the last token: the same bits however far the batch is padded
+        if (l.live && tile == max(l.len - 1, 0) / GS_R) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = h[v];
+            for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = h[v];
+        }
+        if constexpr (W == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) carry[v] = h[v];
+        }
     }
 }
 
@@ -169,12 +431,18 @@ __global__ __launch_bounds__(64) void gs_fwd(GsArgs a) {
 // again from the one kept before it, then
 //   g_t = dy_t silu(z_t) + c,  c = (1-k_t) g_t for the token before
 //   dx = g k, dr = g (h_{t-1} - x) k (1-k), dz = dy h silu'(z)
+// The chain carries c, from the last tile to the first. Kept codes are decoded as
+// they are loaded, to bf16, in which they are exact.
 // ---------------------------------------------------------------------------
-template <class E, int V, int P, bool KEEP>
-__global__ __launch_bounds__(64) void gs_bwd(GsArgs a) {
-    typedef GsVec<E, V> vec;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 64 + lane;
+template <class E, int V, int P, bool KEEP, int W>
+__global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(GsArgs a) {
+    typedef GsPack<E, V> pack;
+    typedef typename std::conditional<KEEP, C8Bf16, E>::type K;  // type of the kept projection in registers
+    __shared__ GsChain<V, W> chain;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    int cg, j, end;
+    gs_place<V, W>(a, chain, cg, j, end);
+    const int64_t id = (int64_t)cg * 64 + lane;
     const GsLane l = gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;
     const int64_t row0 = (int64_t)l.b * a.T;
@@ -182,75 +450,163 @@ __global__ __launch_bounds__(64) void gs_bwd(GsArgs a) {
     const typename E::store* dy = (const typename E::store*)a.dy + l.b * a.dsb + l.d;
     typename E::store* dp = (typename E::store*)a.dp + row0 * P * a.D + l.d;
 
-    float c[V];
+    float carry[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) c[v] = a.dh_last != nullptr ? a.dh_last[(int64_t)l.b * a.D + l.d + v] : 0.f;
+    for (int v = 0; v < V; ++v) carry[v] = a.dh_last != nullptr ? a.dh_last[(int64_t)l.b * a.D + l.d + v] : 0.f;
 
-    for (int tile = nT - 1; tile >= 0; --tile) {
-        const int t0 = tile * GS_R;
-        float val[P][GS_R][V];
-        vec raw_dy[GS_R];
+    for (; j < end; ++j) {
+        const int tile = (a.nJ - 1 - j) * W + wid, t0 = tile * GS_R;
+        GsPack<K, V> raw[P][GS_R];
+        pack up[GS_R];
+        if constexpr (KEEP) {
+            // lane i of 16 has the scale of token i
+            float step[P];
+            const int ti = min(t0 + (lane & 15), a.T - 1);
+            const int ng = a.Dp / C8_GROUP;
+            const int dd = (int)(id % a.tps) * V;  // the group's lanes stay together, padding included
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
-            const int t = min(t0 + i, a.T - 1);
-            raw_dy[i] = *(const vec*)(dy + (int64_t)t * a.dst);
+            for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[((row0 + ti) * P + q) * ng + dd / C8_GROUP]);
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-                if constexpr (KEEP) {
-                    const int64_t row = (row0 + t) * P + q;
-                    const float step = c8_step(a.scales[row * (a.Dp / C8_GROUP) + l.d / C8_GROUP]);
+            for (int i = 0; i < GS_R; ++i) {
+                const int t = min(t0 + i, a.T - 1);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) val[q][i][v] = (float)a.codes[row * a.Dp + l.d + v] * step;
-                } else {
-                    const vec w = *(const vec*)(p + (int64_t)t * a.st + q * a.D);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) val[q][i][v] = E::up(w.v[v]);
+                for (int q = 0; q < P; ++q) {
+                    const signed char* from = a.codes + ((row0 + t) * P + q) * a.Dp + dd;
+                    if constexpr (V == 2) raw[q][i].w = *(const unsigned short*)from;
+                    else raw[q][i].w = *(const unsigned char*)from;
                 }
             }
-        }
-        float h[V], before[GS_R][V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v];
+            for (int i = 0; i < GS_R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
+            gs_for<GS_R>([&](auto n) {
+                constexpr int i = decltype(n)::value;
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    raw[q][i].pin();
+                    // row_newbcast: lane i's value to its 16 lanes
+                    const float s = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(step[q]), 0x150 + i, 0xF, 0xF, true));
+                    const unsigned int w = raw[q][i].w;
+                    const float f0 = (float)(signed char)(w & 0xff) * s;
+                    if constexpr (V == 2) raw[q][i].w = (__float_as_uint(f0) >> 16) | (__float_as_uint((float)(signed char)(w >> 8) * s) & 0xffff0000u);
+                    else raw[q][i].w = __float_as_uint(f0) >> 16;
+                }
+            });
+        } else {
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) {
+                const int t = min(t0 + i, a.T - 1);
+                up[i].load(dy + (int64_t)t * a.dst);
+#pragma unroll
+                for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
+            }
+        }
+        float h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = a.states[((int64_t)l.b * nT + min(tile, nT - 1)) * a.D + l.d + v];
+        float k[GS_R][V], c[V];
+        float2 m[V];
+        const bool whole = __all(l.len >= t0 + GS_R);
+        auto gates = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
+#pragma unroll
+            for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+#pragma unroll
+            for (int i = GS_R - 1; i >= 0; --i) {
+                const bool in = FULL || t0 + i < l.len;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                    if constexpr (W > 1) {
+                        float g = up[i].get(v);
+                        if constexpr (P == 3) {
+                            const float z = raw[2][i].get(v);
+                            g *= z * gs_sigmoid(z);
+                        }
+                        g += m[v].y;
+                        m[v].y = in ? fmaf(-k[i][v], g, g) : m[v].y;
+                        m[v].x = in ? fmaf(-k[i][v], m[v].x, m[v].x) : m[v].x;
+                    }
+                }
+                gs_fence<W>(i);
+            }
+        };
+        if (whole) gates(std::true_type{});
+        else gates(std::false_type{});
+        gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c);
 #pragma unroll
         for (int i = 0; i < GS_R; ++i) {
-            const bool in = t0 + i < l.len;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                before[i][v] = h[v];
-                val[1][i][v] = gs_sigmoid(-val[1][i][v]);  // from here on k
-                h[v] = in ? fmaf(val[1][i][v], val[0][i][v] - h[v], h[v]) : h[v];
-            }
+            raw[P - 1][i].pin();
+            up[i].pin();
         }
+        auto run = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
+            // the states of half a tile at a time: the first half's are computed twice
+            // (two operations each), and half of them in registers is enough
+            constexpr int HALF = GS_R / 2;
+            float first[V], before[HALF][V];
 #pragma unroll
-        for (int i = GS_R - 1; i >= 0; --i) {
-            const bool in = t0 + i < l.len;
-            vec out[P];
+            for (int v = 0; v < V; ++v) first[v] = h[v];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float x = val[0][i][v], k = val[1][i][v], hp = before[i][v];
-                float g = E::up(raw_dy[i].v[v]);
-                if constexpr (P == 3) {
-                    const float z = val[2][i][v];
-                    const float s = gs_sigmoid(z), zs = z * s;
-                    const float hn = fmaf(k, x - hp, hp);
-                    out[2].v[v] = E::down(in ? g * hn * fmaf(zs, 1.f - s, s) : 0.f);
-                    g *= zs;
+            for (int i = 0; i < HALF; ++i) {
+                const bool in = FULL || t0 + i < l.len;
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
+            }
+#pragma unroll
+            for (int half = 1; half >= 0; --half) {
+#pragma unroll
+                for (int n = 0; n < HALF; ++n) {
+                    const int i = half * HALF + n;
+                    const bool in = FULL || t0 + i < l.len;
+                    raw[0][i].pin();
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        before[n][v] = h[v];
+                        h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
+                    }
                 }
-                g += c[v];
-                const float gk = g * k;
-                c[v] = in ? g - gk : c[v];
-                out[0].v[v] = E::down(in ? gk : 0.f);
-                out[1].v[v] = E::down(in ? (hp - x) * fmaf(-k, gk, gk) : 0.f);
-            }
-            if (l.live && t0 + i < a.T) {
 #pragma unroll
-                for (int q = 0; q < P; ++q) *(vec*)(dp + ((int64_t)(t0 + i) * P + q) * a.D) = out[q];
+                for (int n = HALF - 1; n >= 0; --n) {
+                    const int i = half * HALF + n;
+                    const bool in = FULL || t0 + i < l.len;
+                    float out[P][V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float x = raw[0][i].get(v), kk = k[i][v], hp = before[n][v];
+                        float g = up[i].get(v);
+                        if constexpr (P == 3) {
+                            const float z = raw[2][i].get(v);
+                            const float s = gs_sigmoid(z), zs = z * s;
+                            const float hn = fmaf(kk, x - hp, hp);
+                            out[2][v] = in ? g * hn * fmaf(zs, 1.f - s, s) : 0.f;
+                            g *= zs;
+                        }
+                        g += c[v];
+                        const float gk = g * kk;
+                        c[v] = in ? g - gk : c[v];
+                        out[0][v] = in ? gk : 0.f;
+                        out[1][v] = in ? (hp - x) * fmaf(-kk, gk, gk) : 0.f;
+                    }
+                    if (l.live && (FULL || t0 + i < a.T)) {
+#pragma unroll
+                        for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)(t0 + i) * P + q) * a.D, out[q]);
+                    }
+                    gs_fence<W>(i);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = first[v];
             }
+        };
+        if (whole) run(std::true_type{});
+        else run(std::false_type{});
+        if (l.live && a.dh0 != nullptr && tile == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) a.dh0[(int64_t)l.b * a.D + l.d + v] = c[v];
         }
-    }
-    if (l.live && a.dh0 != nullptr) {
+        if constexpr (W == 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) a.dh0[(int64_t)l.b * a.D + l.d + v] = c[v];
+            for (int v = 0; v < V; ++v) carry[v] = c[v];
+        }
     }
 }
 
@@ -278,15 +634,13 @@ __device__ __forceinline__ int64_t gs_slot(const GsStepArgs& a, int b) {
 
 template <class E, int V, int P>
 __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
-    typedef GsVec<E, V> vec;
+    typedef GsPack<E, V> pack;
     const int row = blockIdx.x;
     const int64_t slot = a.slots != nullptr ? gs_slot(a, row) : row;
     typename E::store* y = (typename E::store*)a.y;
     if (slot < 0 || slot >= a.S) {  // no state: a row of padding
-        vec zero;
-#pragma unroll
-        for (int v = 0; v < V; ++v) zero.v[v] = E::down(0.f);
-        for (int d = threadIdx.x * V; d < a.D; d += blockDim.x * V) *(vec*)(y + (int64_t)row * a.D + d) = zero;
+        const float zero[V] = {};
+        for (int d = threadIdx.x * V; d < a.D; d += blockDim.x * V) pack::put(y + (int64_t)row * a.D + d, zero);
         return;
     }
     int later = 0;
@@ -308,20 +662,20 @@ __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
         for (int b = row; b < a.B; ++b) {
             if (b != row && gs_slot(a, b) != slot) continue;
             const typename E::store* p = (const typename E::store*)a.p + b * a.sb + d;
-            vec raw[P], out;
+            pack raw[P];
+            float out[V];
 #pragma unroll
-            for (int q = 0; q < P; ++q) raw[q] = *(const vec*)(p + (int64_t)q * a.D);
+            for (int q = 0; q < P; ++q) raw[q].load(p + (int64_t)q * a.D);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = fmaf(gs_sigmoid(-E::up(raw[1].v[v])), E::up(raw[0].v[v]) - h[v], h[v]);
-                float o = h[v];
+                h[v] = fmaf(gs_sigmoid(-raw[1].get(v)), raw[0].get(v) - h[v], h[v]);
+                out[v] = h[v];
                 if constexpr (P == 3) {
-                    const float z = E::up(raw[2].v[v]);
-                    o *= z * gs_sigmoid(z);
+                    const float z = raw[2].get(v);
+                    out[v] *= z * gs_sigmoid(z);
                 }
-                out.v[v] = E::down(o);
             }
-            *(vec*)(y + (int64_t)b * a.D + d) = out;
+            pack::put(y + (int64_t)b * a.D + d, out);
             if (!later) break;
         }
 #pragma unroll
@@ -329,19 +683,22 @@ __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
     }
 }
 
-bool gs_pairs(const torch::Tensor& t) {
-    return ((uintptr_t)t.data_ptr() % (2 * t.element_size())) == 0;
-}
+// a lane takes two neighbouring channels where that is one aligned 32-bit access
+bool gs_pairs(const torch::Tensor& t) { return t.element_size() == 2 && (uintptr_t)t.data_ptr() % 4 == 0; }
 
 // calls f.template operator()<E, V, P>()
 template <class F>
 void gs_types(at::ScalarType dt, bool pair, int64_t parts, F&& f) {
     auto with = [&](auto e) {
         typedef decltype(e) E;
-        if (pair) {
-            if (parts == 3) f.template operator()<E, 2, 3>();
-            else f.template operator()<E, 2, 2>();
-        } else {
+        if constexpr (sizeof(typename E::store) == 2) {
+            if (pair) {
+                if (parts == 3) f.template operator()<E, 2, 3>();
+                else f.template operator()<E, 2, 2>();
+                return;
+            }
+        }
+        {
             if (parts == 3) f.template operator()<E, 1, 3>();
             else f.template operator()<E, 1, 2>();
         }
@@ -357,27 +714,71 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
                 "gated_scan: ", what, " must be contiguous float32 with ", n, " values on the device of p");
 }
 
+// How a scan is laid out. One wave a block that walks all tokens (W = 1) needs no
+// exchange, and fills the chip from 2048 groups of channels on (8 waves a CU). With
+// fewer, `many` waves share the tokens; with fewer than two such blocks a CU,
+// and more than a few tiles, blocks are chained along time. Forward without codes
+// fits 128 registers a lane: blocks of 8 waves, 4 waves a SIMD. The codes and the
+// backward pass need up to 168: blocks of 4, 3 waves a SIMD.
+struct GsPlan {
+    int W;
+    unsigned int blocks;
+    torch::Tensor space;
+};
+
+GsPlan gs_plan(GsArgs& a, int V, int many, const torch::Tensor& p, hipStream_t stream) {
+    GsPlan plan;
+    const int64_t groups = ((int64_t)a.B * a.tps + 63) / 64;
+    TORCH_CHECK(groups <= INT_MAX && a.T <= (1 << 30), "gated_scan: sizes of p out of range");
+    plan.W = a.T <= GS_R || groups >= 2048 ? 1 : many;
+    a.groups = (int)groups;
+    a.nJ = (a.T + plan.W * GS_R - 1) / (plan.W * GS_R);
+    int64_t blocks = groups;
+    if (plan.W > 1 && groups < 512 && a.nJ > 4) {
+        blocks = groups * a.nJ;
+        const int64_t words = blocks * V * 64, links = (int64_t)((a.nJ + GS_LB - 1) / GS_LB) * groups * V * 64;
+        const int64_t n = (words * 8 + links * 4 + 16 + 15) / 16;
+        plan.space = torch::empty({n * 16}, p.options().dtype(at::kByte));
+        char* at = (char*)plan.space.data_ptr();
+        a.ticket = (unsigned int*)at;
+        a.agg = (unsigned long long*)(at + 16);
+        a.prefix = (unsigned int*)(at + 16 + words * 8);
+        hipLaunchKernelGGL(gs_clear, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, stream, (uint4*)at, n);
+    }
+    TORCH_CHECK(blocks <= INT_MAX, "gated_scan: too many blocks");
+    plan.blocks = (unsigned int)blocks;
+    return plan;
+}
+
 struct GsFwdCall {
     const GsArgs& a;
-    int64_t blocks;
+    const GsPlan& plan;
     hipStream_t stream;
-    bool keep;
+    template <class E, int V, int P, bool KEEP>
+    void with() {
+        if (plan.W == 1) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        else hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, KEEP ? 4 : 8>), dim3(plan.blocks), dim3(KEEP ? 256 : 512), 0, stream, a);
+    }
     template <class E, int V, int P>
     void operator()() {
-        if (keep) hipLaunchKernelGGL((gs_fwd<E, V, P, true>), dim3((unsigned)blocks), dim3(64), 0, stream, a);
-        else hipLaunchKernelGGL((gs_fwd<E, V, P, false>), dim3((unsigned)blocks), dim3(64), 0, stream, a);
+        if (a.codes != nullptr) with<E, V, P, true>();
+        else with<E, V, P, false>();
     }
 };
 
 struct GsBwdCall {
     const GsArgs& a;
-    int64_t blocks;
+    const GsPlan& plan;
     hipStream_t stream;
-    bool keep;
+    template <class E, int V, int P, bool KEEP>
+    void with() {
+        if (plan.W == 1) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        else hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 4>), dim3(plan.blocks), dim3(256), 0, stream, a);
+    }
     template <class E, int V, int P>
     void operator()() {
-        if (keep) hipLaunchKernelGGL((gs_bwd<E, V, P, true>), dim3((unsigned)blocks), dim3(64), 0, stream, a);
-        else hipLaunchKernelGGL((gs_bwd<E, V, P, false>), dim3((unsigned)blocks), dim3(64), 0, stream, a);
+        if (a.codes != nullptr) with<E, V, P, true>();
+        else with<E, V, P, false>();
     }
 };
 
@@ -454,9 +855,9 @@ void gated_scan_fwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
     const int V = pair ? 2 : 1;
     a.tps = a.codes != nullptr ? a.Dp / V : a.D / V;
     const c10::DeviceGuard guard(p.device());
-    const int64_t blocks = ((int64_t)a.B * a.tps + 63) / 64;
-    TORCH_CHECK(blocks <= INT_MAX, "gated_scan: too many channels");
-    GsFwdCall call{a, blocks, at::hip::getCurrentHIPStream().stream(), a.codes != nullptr};
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    const GsPlan plan = gs_plan(a, V, a.codes != nullptr ? 4 : 8, p, stream);
+    GsFwdCall call{a, plan, stream};
     gs_types(p.scalar_type(), pair, parts, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -493,11 +894,12 @@ void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
     gs_codes(a, codes, scales, p, parts);
     const bool pair = a.D % 2 == 0 && a.dsb % 2 == 0 && a.dst % 2 == 0 && gs_pairs(dy) && gs_pairs(dp) &&
                       (a.codes != nullptr || (a.sb % 2 == 0 && a.st % 2 == 0 && gs_pairs(p)));
-    a.tps = a.D / (pair ? 2 : 1);
+    const int V = pair ? 2 : 1;
+    a.tps = a.codes != nullptr ? a.Dp / V : a.D / V;
     const c10::DeviceGuard guard(p.device());
-    const int64_t blocks = ((int64_t)a.B * a.tps + 63) / 64;
-    TORCH_CHECK(blocks <= INT_MAX, "gated_scan: too many channels");
-    GsBwdCall call{a, blocks, at::hip::getCurrentHIPStream().stream(), a.codes != nullptr};
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    const GsPlan plan = gs_plan(a, V, 4, p, stream);
+    GsBwdCall call{a, plan, stream};
     gs_types(p.scalar_type(), pair, parts, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();
 }

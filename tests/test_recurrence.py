@@ -39,46 +39,40 @@ def definition(p, dim, h0, lengths, dy, dh, keep="input"):
     """(y, h_last, dp, dh0) in float64 on the CPU, token by token."""
     p, dy, dh = (t.detach().cpu().double() for t in (p, dy, dh))
     B, T, width = p.shape
-    h0 = torch.zeros(B, dim, dtype=torch.float64) if h0 is None else h0.detach().cpu().double()
-    n = [T] * B if lengths is None else [min(max(int(v), 0), T) for v in lengths.cpu()]
-    y = torch.zeros(B, T, dim, dtype=torch.float64)
-    dp = torch.zeros_like(p)
-    last, dh0 = h0.clone(), dh.clone()
-    for b in range(B):
-        h, states = h0[b], []
-        for t in range(n[b]):
-            states.append(h)
-            x, r = p[b, t, :dim], p[b, t, dim : 2 * dim]
-            f = torch.sigmoid(r)
-            h = f * h + (1 - f) * x
-            y[b, t] = h
-            if width == 3 * dim:
-                z = p[b, t, 2 * dim :]
-                y[b, t] = h * z * torch.sigmoid(z)
-        last[b] = h
-        q = p[b]
-        if keep == "int8":
-            q = torch.cat([kept8(part) for part in p[b].split(dim, -1)], -1)
-            for t in range(n[b]):
-                if t % EVERY:
-                    f = torch.sigmoid(q[t - 1, dim : 2 * dim])
-                    states[t] = f * states[t - 1] + (1 - f) * q[t - 1, :dim]
-        c = dh[b]
-        for t in range(n[b] - 1, -1, -1):
-            x, f = q[t, :dim], torch.sigmoid(q[t, dim : 2 * dim])
-            g = dy[b, t]
-            if width == 3 * dim:
-                z = q[t, 2 * dim :]
-                s = torch.sigmoid(z)
-                h = f * states[t] + (1 - f) * x
-                dp[b, t, 2 * dim :] = g * h * (s + z * s * (1 - s))
-                g = g * z * s
-            g = g + c
-            dp[b, t, :dim] = g * (1 - f)
-            dp[b, t, dim : 2 * dim] = g * (states[t] - x) * f * (1 - f)
-            c = g * f
-        dh0[b] = c
-    return y, last, dp, dh0
+    h = torch.zeros(B, dim, dtype=torch.float64) if h0 is None else h0.detach().cpu().double()
+    n = torch.full((B, 1), T) if lengths is None else lengths.cpu().long().clamp(0, T)[:, None]
+    y, dp = torch.zeros(B, T, dim, dtype=torch.float64), torch.zeros_like(p)
+    states = []
+    for t in range(T):
+        states.append(h)
+        x, f = p[:, t, :dim], torch.sigmoid(p[:, t, dim : 2 * dim])
+        h = torch.where(t < n, f * h + (1 - f) * x, h)
+        out = h
+        if width == 3 * dim:
+            z = p[:, t, 2 * dim :]
+            out = h * z * torch.sigmoid(z)
+        y[:, t] = torch.where(t < n, out, 0.0)
+    last, q = h, p
+    if keep == "int8":
+        q = torch.cat([kept8(part) for part in p.split(dim, -1)], -1)
+        for t in range(T):
+            if t % EVERY:
+                f = torch.sigmoid(q[:, t - 1, dim : 2 * dim])
+                states[t] = f * states[t - 1] + (1 - f) * q[:, t - 1, :dim]
+    c = dh
+    for t in range(T - 1, -1, -1):
+        x, f = q[:, t, :dim], torch.sigmoid(q[:, t, dim : 2 * dim])
+        g, parts = dy[:, t], []
+        if width == 3 * dim:
+            z = q[:, t, 2 * dim :]
+            s = torch.sigmoid(z)
+            parts = [g * (f * states[t] + (1 - f) * x) * (s + z * s * (1 - s))]
+            g = g * z * s
+        g = g + c
+        parts = [g * (1 - f), g * (states[t] - x) * f * (1 - f)] + parts
+        dp[:, t] = torch.where(t < n, torch.cat(parts, -1), 0.0)
+        c = torch.where(t < n, g * f, c)
+    return y, last, dp, c
 
 
 def inputs(B, T, D, dtype, device, gate=True, seed=0):
@@ -360,6 +354,50 @@ def test_step_refuses():
 
 
 # ------------------------------------------------------------- on the GPU alone
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "plain"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize(
+    "B,T,D",
+    [
+        (1, 513, 64),     # time split over blocks that are chained
+        (1, 2049, 40),    # the chain's first link, forward, and a lone token behind it
+        (2, 5000, 33),    # many links, lanes that straddle two sequences
+        (1, 4097, 1),     # one channel
+        (5, 1100, 130),
+        (700, 150, 50),   # a block walks several tiles
+        (600, 650, 120),  # many of them
+        (2200, 70, 62),   # a wave walks alone
+        (70000, 3, 4),    # a tile is more than a sequence
+    ],
+)
+def test_every_way_of_splitting(B, T, D, dtype, gate, keep):
+    p, h0, dy, dh = inputs(B, T, D, dtype, "cuda", gate)
+    lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(2)).cuda()
+    lengths[-1] = T
+    check(p, D, h0, lengths, dy, dh, keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,D", [(3000, 32), (3000, 8192)])
+def test_nan_goes_where_it_belongs(T, D):
+    """A NaN of any bits in one channel of one token: that channel from there on,
+    and its gradient up to there; the chain between blocks waits for no such word."""
+    p, h0, dy, dh = inputs(1, T, D, torch.float32, "cuda", gate=False)
+    p[0, 100, 5] = torch.tensor(-1, dtype=torch.int32).view(torch.float32)
+    q = p.clone().requires_grad_()
+    y, last = gated_scan(q, D, h0)
+    bad = y[0].isnan()
+    assert not bad[:100].any() and bad[100:, 5].all() and int(bad.sum()) == T - 100
+    assert last[0, 5].isnan() and int(last.isnan().sum()) == 1
+    dyn = dy.clone()
+    dyn[0, T - 50, 7] = torch.tensor(-1, dtype=torch.int32).view(torch.float32)
+    q = inputs(1, T, D, torch.float32, "cuda", gate=False)[0].requires_grad_()
+    dp = torch.autograd.grad(gated_scan(q, D, h0), q, (dyn, dh))[0][0, :, :D].isnan()
+    assert dp[: T - 49, 7].all() and int(dp.sum()) == T - 49
+
+
 @pytest.mark.gpu
 def test_same_inputs_same_bits():
     p, h0, dy, dh = inputs(2, 700, 96, torch.bfloat16, "cuda")
