@@ -55,7 +55,7 @@ __device__ __forceinline__ unsigned int c8_scale(unsigned int top) {
     return field == 255u ? 255u : (field > 7u ? field - 6u : 1u);
 }
 
-// 2^-e of a scale byte; 0 for a group that is not finite, so that its codes are 0
+// 2^-e of a scale byte; 0 for a group that is not finite
 __device__ __forceinline__ float c8_inv(unsigned int s) {
     return s == 255u ? 0.f : __uint_as_float((254u - s) << 23);
 }
@@ -65,10 +65,12 @@ __device__ __forceinline__ float c8_step(unsigned int s) {
     return s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23);
 }
 
-__device__ __forceinline__ int c8_code(float v, float inv) {
-    float q = rintf(v * inv);           // v * inv is exact; a NaN product is caught below
-    q = fminf(fmaxf(q, -127.f), 127.f); // fmaxf(NaN, a) is a
-    return inv == 0.f ? 0 : (int)q;
+// The code as a byte. v * inv is exact; added to 1.5 * 2^23 it is rounded to the
+// nearest integer, ties to even, and its two's complement is in the low bits. In a
+// group that is not finite (inv = 0) a code means nothing.
+__device__ __forceinline__ unsigned int c8_code_byte(float v, float inv) {
+    const float q = __builtin_amdgcn_fmed3f(fmaf(v, inv, 12582912.f), 12582912.f - 127.f, 12582912.f + 127.f);
+    return __float_as_uint(q) & 0xffu;
 }
 
 // max over 16 lanes of a row (DPP: no LDS pass)

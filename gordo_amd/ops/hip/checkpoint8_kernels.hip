@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void c8_save(const typename E::store* x, int64
         const float b = col + 1 < F ? E::up(x[row * sx + col + 1]) : 0.f;
         const unsigned int s = c8_scale(c8_max16(max(c8_mag(a), c8_mag(b))));
         const float inv = c8_inv(s);
-        *(short*)(codes + row * Fp + col) = (short)((c8_code(a, inv) & 0xff) | (c8_code(b, inv) << 8));
+        *(unsigned short*)(codes + row * Fp + col) = (unsigned short)(c8_code_byte(a, inv) | (c8_code_byte(b, inv) << 8));
         if (col % C8_GROUP == 0) scales[row * ng + col / C8_GROUP] = (unsigned char)s;
     }
 }

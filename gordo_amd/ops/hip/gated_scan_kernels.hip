@@ -54,6 +54,17 @@ struct GsPack {
     }
 };
 
+// A token behind its sequence's end: shut gate (r = +inf, so k = 0 and the state and
+// the gradient pass through), nothing in x and z. Whatever p holds there is gone
+// before it is used, and the loops over a tile need no masks.
+template <class E, int V, int P>
+__device__ __forceinline__ void gs_mask(GsPack<E, V> (&raw)[P][GS_R], int i, bool out) {
+    const unsigned int inf = sizeof(typename E::store) == 4 ? 0x7f800000u : (std::is_same<E, C8Bf16>::value ? 0x7f80u : 0x7c00u) * (V == 2 ? 0x10001u : 1u);
+    raw[0][i].w = out ? 0u : raw[0][i].w;
+    raw[1][i].w = out ? inf : raw[1][i].w;
+    if constexpr (P == 3) raw[2][i].w = out ? 0u : raw[2][i].w;
+}
+
 // Where waves share a CU by registers, a scheduler that interleaves many tokens to
 // hide latencies spills: two tokens at a time are enough beside the other waves.
 template <int W>
@@ -154,6 +165,12 @@ __device__ __forceinline__ float2 gs_then(float2 first, float2 second) {
     return float2{first.x * second.x, fmaf(second.x, first.y, second.y)};
 }
 
+// another look at a word that was not there; false: give up
+__device__ __forceinline__ bool gs_again(int& spins) {
+    __builtin_amdgcn_s_sleep(1);
+    return ++spins < GS_SPINS;
+}
+
 template <int V, int W>
 struct GsChain {
     float2 part[2][W][V][64];
@@ -173,7 +190,7 @@ __device__ __forceinline__ void gs_place(const GsArgs& a, GsChain<V, W>& s, int&
         if (a.ticket != nullptr) {
             if (threadIdx.x == 0) s.ticket = atomicAdd(a.ticket, 1u) + 1u;  // it starts at all ones
             __syncthreads();
-            const unsigned int t = s.ticket;
+            const unsigned int t = __builtin_amdgcn_readfirstlane(s.ticket);
             j = (int)(t / (unsigned int)a.groups);
             cg = (int)(t - (unsigned int)j * a.groups);
             end = j + 1;
@@ -182,8 +199,8 @@ __device__ __forceinline__ void gs_place(const GsArgs& a, GsChain<V, W>& s, int&
 }
 
 // The state that enters this wave's tile, from `carry` (the state that enters the
-// block's first tile; of the chain's first block where blocks are chained), and in
-// `carry` the state after the block's last tile. `mine`: this wave's map; `order`:
+// block's first tile; of the chain's first block where blocks are chained), and,
+// where a block walks on, in `carry` the state after its last tile. `mine`: this wave's map; `order`:
 // this wave's place in the block, 0 first. j counts tiles in the chain's order.
 template <int V, int W>
 __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int cg, int j, int order, int lane,
@@ -197,88 +214,95 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
 #pragma unroll
     for (int v = 0; v < V; ++v) s.part[par][order][v][lane] = mine[v];
     __syncthreads();
-    if (a.ticket != nullptr) {
-        const int i = j % GS_LB, g = j / GS_LB;
-        const bool more = j + 1 < a.nJ;
-        if (order == W - 1 && i < GS_LB - 1 && more) {
+    // the map from the block's first state to this wave's, and to the one after the block
+    float2 to[V], all[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float2 m = s.part[par][0][v][lane];
+    for (int v = 0; v < V; ++v) all[v] = float2{1.f, 0.f};
+    const auto parts = [&] {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
 #pragma unroll 2
-                for (int w = 1; w < W; ++w) m = gs_then(m, s.part[par][w][v][lane]);
-                gs_publish(a.agg + (((int64_t)j * a.groups + cg) * V + v) * 64 + lane, m);
+            for (int w = 0; w < W; ++w) {
+                if (w == order) to[v] = all[v];
+                all[v] = gs_then(all[v], s.part[par][w][v][lane]);
             }
         }
-        // the wave's share of the blocks before: all loads go out, then all are looked at
-        const int Q = (GS_LB + W - 1) / W;
-        unsigned long long word[Q][V];
-        unsigned int first[V];
-        const bool chained = order == 0 && g > 0;
+    };
+    if (a.ticket == nullptr) {
+        parts();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            in[v] = fmaf(to[v].x, carry[v], to[v].y);
+            carry[v] = fmaf(all[v].x, carry[v], all[v].y);
+        }
+        return;
+    }
+    const int i = j % GS_LB, g = j / GS_LB;
+    const bool more = j + 1 < a.nJ;
+    if (order == W - 1 && i < GS_LB - 1 && more) {
+        parts();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            gs_publish(a.agg + (((int64_t)j * a.groups + cg) * V + v) * 64 + lane, all[v]);
+            all[v] = float2{1.f, 0.f};
+        }
+    }
+    // the wave's share of the blocks before, since the last link
+    int spins = 0;
+    for (int q = order; q < i; q += W) {
+        unsigned long long word[V];
+        const unsigned long long* from = a.agg + ((int64_t)(g * GS_LB + q) * a.groups + cg) * V * 64 + lane;
         bool there;
-        int spins = 0;
         do {
             there = true;
 #pragma unroll
-            for (int q = 0; q < Q; ++q)
+            for (int v = 0; v < V; ++v) word[v] = __hip_atomic_load(from + v * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (q * W + order < i)
-                        word[q][v] = __hip_atomic_load(a.agg + (((int64_t)(g * GS_LB + q * W + order) * a.groups + cg) * V + v) * 64 + lane,
-                                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (chained) {
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    first[v] = __hip_atomic_load(a.prefix + (((int64_t)(g - 1) * a.groups + cg) * V + v) * 64 + lane,
-                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-#pragma unroll
-            for (int q = 0; q < Q; ++q)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (q * W + order < i) there &= (unsigned int)word[q][v] != ~0u;
-            if (chained) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) there &= first[v] != ~0u;
-            }
-        } while (!__all(there) && ++spins < GS_SPINS);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q)
-                if (q * W + order < i)
-                    s.pred[q * W + order][v][lane] = float2{__uint_as_float((unsigned int)word[q][v]),
-                                                            __uint_as_float((unsigned int)(word[q][v] >> 32))};
-            if (order == 0) s.start[v][lane] = chained ? __uint_as_float(first[v]) : carry[v];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float h = s.start[v][lane];
-#pragma unroll 2
-            for (int q = 0; q < i; ++q) {
-                const float2 m = s.pred[q][v][lane];
-                h = fmaf(m.x, h, m.y);
-            }
-            carry[v] = h;
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float h = carry[v];
-#pragma unroll 2
-        for (int w = 0; w < W; ++w) {
-            if (w == order) in[v] = h;
-            const float2 m = s.part[par][w][v][lane];
-            h = fmaf(m.x, h, m.y);
-        }
-        carry[v] = h;
-    }
-    if (a.ticket != nullptr && order == W - 1 && j % GS_LB == GS_LB - 1 && j + 1 < a.nJ) {
+            for (int v = 0; v < V; ++v) there &= (unsigned int)word[v] != ~0u;
+        } while (!__all(there) && gs_again(spins));
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            __hip_atomic_store(a.prefix + (((int64_t)(j / GS_LB) * a.groups + cg) * V + v) * 64 + lane, gs_word(carry[v]),
-                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.pred[q][v][lane] = float2{__uint_as_float((unsigned int)word[v]), __uint_as_float((unsigned int)(word[v] >> 32))};
     }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll 2
+        for (int q = 0; q < i; ++q) all[v] = gs_then(all[v], s.pred[q][v][lane]);
+    }
+    parts();
+    // All maps are ready before the state that they are applied to is there: from a
+    // link to the next it is one load, one operation and one store.
+    if (order == W - 1) {
+        float start[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) start[v] = carry[v];
+        if (g > 0) {
+            unsigned int word[V];
+            const unsigned int* from = a.prefix + ((int64_t)(g - 1) * a.groups + cg) * V * 64 + lane;
+            bool there;
+            do {
+                there = true;
+#pragma unroll
+                for (int v = 0; v < V; ++v) word[v] = __hip_atomic_load(from + v * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int v = 0; v < V; ++v) there &= word[v] != ~0u;
+            } while (!__all(there) && gs_again(spins));
+#pragma unroll
+            for (int v = 0; v < V; ++v) start[v] = __uint_as_float(word[v]);
+        }
+        if (i == GS_LB - 1 && more) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                __hip_atomic_store(a.prefix + (((int64_t)g * a.groups + cg) * V + v) * 64 + lane,
+                                   gs_word(fmaf(all[v].x, start[v], all[v].y)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) s.start[v][lane] = start[v];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) in[v] = fmaf(to[v].x, s.start[v][lane], to[v].y);
 }
 
 // all ones: no word of the chain is there yet, and the next ticket is 0
@@ -291,34 +315,37 @@ __global__ __launch_bounds__(256) void gs_clear(uint4* to, int64_t n) {
 // ---------------------------------------------------------------------------
 
 // The codes and scales of a tile of one part. The 32 values of a group are pairs
-// in 16 lanes (V = 2) or one in each of 32 (V = 1); a tile has 16 tokens, so
-// lane i of 16 collects the scale of token i and stores it once.
+// in 16 lanes (V = 2) or one in each of 32 (V = 1). A tile has 16 tokens: lane i of
+// 16 takes the largest magnitude of token i, so the scales of all tokens are made
+// at once and stored once, and come back to the lanes by a broadcast.
 template <class E, int V>
 __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&raw)[GS_R], bool live, bool mine, int64_t row,
                                           int64_t step, int left, int dd, int lane) {
-    unsigned int scale = 0;
-    signed char* to = a.codes + row * a.Dp + dd;
+    unsigned int top = 0;
 #pragma unroll
     for (int i = 0; i < GS_R; ++i) {
-        float f[V];
-        unsigned int top = 0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            f[v] = live ? raw[i].get(v) : 0.f;
-            top = max(top, c8_mag(f[v]));
-        }
-        top = c8_max16(top);
-        if constexpr (V == 1) top = max(top, (unsigned int)__shfl_xor((int)top, 16, 64));
-        const unsigned int s = c8_scale(top);
-        const float inv = c8_inv(s);
-        scale = (lane & 15) == i ? s : scale;
+        unsigned int t = c8_mag(raw[i].get(0));
+        if constexpr (V == 2) t = max(t, c8_mag(raw[i].get(1)));
+        t = c8_max16(live ? t : 0u);
+        if constexpr (V == 1) t = max(t, (unsigned int)__shfl_xor((int)t, 16, 64));
+        top = (lane & 15) == i ? t : top;
+    }
+    const unsigned int scale = c8_scale(top);
+    const float mine_inv = c8_inv(scale);
+    signed char* to = a.codes + row * a.Dp + dd;
+    gs_for<GS_R>([&](auto n) {
+        constexpr int i = decltype(n)::value;
+        // row_newbcast: lane i's value to its 16 lanes
+        const float inv = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(mine_inv), 0x150 + i, 0xF, 0xF, true));
+        unsigned int c = c8_code_byte(live ? raw[i].get(0) : 0.f, inv);
+        if constexpr (V == 2) c |= c8_code_byte(live ? raw[i].get(1) : 0.f, inv) << 8;
         if (mine && i < left) {
-            if constexpr (V == 2) *(short*)to = (short)((c8_code(f[0], inv) & 0xff) | (c8_code(f[1], inv) << 8));
-            else to[0] = (signed char)c8_code(f[0], inv);
+            if constexpr (V == 2) *(unsigned short*)to = (unsigned short)c;
+            else *(unsigned char*)to = (unsigned char)c;
         }
         to += step * a.Dp;
-        __builtin_amdgcn_sched_barrier(0);  // one token after the other: interleaved, they need too many registers
-    }
+        if constexpr (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    });
     const int i = lane & 15;
     if (mine && i < left && (V == 2 || (lane & 16) == 0))
         a.scales[(row + i * step) * (a.Dp / C8_GROUP) + dd / C8_GROUP] = (unsigned char)scale;
@@ -328,7 +355,7 @@ template <class E, int V, int P, bool KEEP, int W>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(GsArgs a) {
     typedef GsPack<E, V> pack;
     __shared__ GsChain<V, W> chain;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
@@ -350,31 +377,26 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
             for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
         }
+        if (!__all(l.len >= t0 + GS_R)) {
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) gs_mask<E, V, P>(raw, i, t0 + i >= l.len);
+        }
         float k[GS_R][V], h[V];
         float2 m[V];
-        const bool whole = __all(l.len >= t0 + GS_R);  // every token of the tile is one of every lane's sequence
-        auto gates = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-            for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+        for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
-                const bool in = FULL || t0 + i < l.len;
+        for (int i = 0; i < GS_R; ++i) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    k[i][v] = gs_sigmoid(-raw[1][i].get(v));
-                    if constexpr (W > 1) {
-                        const float x = raw[0][i].get(v);
-                        // selected, not multiplied by 0: padding may hold anything
-                        m[v].y = in ? fmaf(k[i][v], x - m[v].y, m[v].y) : m[v].y;
-                        m[v].x = in ? fmaf(-k[i][v], m[v].x, m[v].x) : m[v].x;
-                    }
+            for (int v = 0; v < V; ++v) {
+                k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                if constexpr (W > 1) {
+                    m[v].y = fmaf(k[i][v], raw[0][i].get(v) - m[v].y, m[v].y);
+                    m[v].x = fmaf(-k[i][v], m[v].x, m[v].x);
                 }
-                gs_fence<W>(i);
             }
-        };
-        if (whole) gates(std::true_type{});
-        else gates(std::false_type{});
+            gs_fence<W>(i);
+        }
         gs_join<V, W>(a, chain, cg, j, wid, lane, m, carry, h);
         if (a.states != nullptr && l.live && tile < nT) {
 #pragma unroll
@@ -391,29 +413,25 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             }
         }
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) raw[0][i].pin();
-        auto run = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
+        for (int i = 0; i < GS_R; ++i) {
+            float out[V];
+            raw[0][i].pin();
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
-                const bool in = FULL || t0 + i < l.len;
-                float out[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
-                    out[v] = h[v];
-                    if constexpr (P == 3) {
-                        const float z = raw[2][i].get(v);
-                        out[v] *= z * gs_sigmoid(z);
-                    }
-                    out[v] = in ? out[v] : 0.f;
+            for (int v = 0; v < V; ++v) {
+                h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+                out[v] = h[v];
+                if constexpr (P == 3) {
+                    const float z = raw[2][i].get(v);
+                    out[v] *= z * gs_sigmoid(z);
                 }
-                if (l.live && (FULL || t0 + i < a.T)) pack::put(y + (int64_t)(t0 + i) * a.D, out);
-                gs_fence<W>(i);
             }
-        };
-        if (whole) run(std::true_type{});
-        else run(std::false_type{});
+            if (l.live && t0 + i < l.len) pack::put(y + (int64_t)(t0 + i) * a.D, out);
+            gs_fence<W>(i);
+        }
+        if (l.live) {
+            const float zero[V] = {};
+            for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
+        }
         // from the wave that has the last token: the same bits however far the batch is padded
         if (l.live && tile == max(l.len - 1, 0) / GS_R) {
 #pragma unroll
@@ -439,7 +457,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
     typedef GsPack<E, V> pack;
     typedef typename std::conditional<KEEP, C8Bf16, E>::type K;  // type of the kept projection in registers
     __shared__ GsChain<V, W> chain;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
@@ -503,102 +521,99 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = a.states[((int64_t)l.b * nT + min(tile, nT - 1)) * a.D + l.d + v];
+        if (!__all(l.len >= t0 + GS_R)) {
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) {
+                gs_mask<K, V, P>(raw, i, t0 + i >= l.len);
+                up[i].w = t0 + i >= l.len ? 0u : up[i].w;
+            }
+        }
         float k[GS_R][V], c[V];
         float2 m[V];
-        const bool whole = __all(l.len >= t0 + GS_R);
-        auto gates = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-            for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+        for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
 #pragma unroll
-            for (int i = GS_R - 1; i >= 0; --i) {
-                const bool in = FULL || t0 + i < l.len;
+        for (int i = GS_R - 1; i >= 0; --i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                if constexpr (W > 1) {
+                    float g = up[i].get(v);
+                    if constexpr (P == 3) {
+                        const float z = raw[2][i].get(v);
+                        g *= z * gs_sigmoid(z);
+                    }
+                    g += m[v].y;
+                    m[v].y = fmaf(-k[i][v], g, g);
+                    m[v].x = fmaf(-k[i][v], m[v].x, m[v].x);
+                }
+            }
+            gs_fence<W>(i);
+        }
+        gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c);
+        // the states of half a tile at a time: the first half's are computed twice
+        // (two operations each), and half of them in registers is enough
+        constexpr int HALF = GS_R / 2;
+        float first[V], before[HALF][V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) first[v] = h[v];
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            raw[0][i].pin();
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+        }
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+#pragma unroll
+            for (int n = 0; n < HALF; ++n) {
+                const int i = half * HALF + n;
+                raw[0][i].pin();
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    k[i][v] = gs_sigmoid(-raw[1][i].get(v));
-                    if constexpr (W > 1) {
-                        float g = up[i].get(v);
-                        if constexpr (P == 3) {
-                            const float z = raw[2][i].get(v);
-                            g *= z * gs_sigmoid(z);
-                        }
-                        g += m[v].y;
-                        m[v].y = in ? fmaf(-k[i][v], g, g) : m[v].y;
-                        m[v].x = in ? fmaf(-k[i][v], m[v].x, m[v].x) : m[v].x;
+                    before[n][v] = h[v];
+                    h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+                }
+            }
+            gs_fence<W>(0);
+#pragma unroll
+            for (int n = HALF - 1; n >= 0; --n) {
+                const int i = half * HALF + n;
+                float out[P][V];
+                raw[P - 1][i].pin();
+                up[i].pin();
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float x = raw[0][i].get(v), kk = k[i][v], hp = before[n][v];
+                    float g = up[i].get(v);
+                    if constexpr (P == 3) {
+                        const float z = raw[2][i].get(v);
+                        const float s = gs_sigmoid(z), zs = z * s;
+                        const float hn = fmaf(kk, x - hp, hp);
+                        out[2][v] = g * hn * fmaf(zs, 1.f - s, s);
+                        g *= zs;
                     }
+                    g += c[v];
+                    const float gk = g * kk;
+                    c[v] = g - gk;
+                    out[0][v] = gk;
+                    out[1][v] = (hp - x) * fmaf(-kk, gk, gk);
+                }
+                if (l.live && t0 + i < l.len) {
+#pragma unroll
+                    for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)(t0 + i) * P + q) * a.D, out[q]);
                 }
                 gs_fence<W>(i);
             }
-        };
-        if (whole) gates(std::true_type{});
-        else gates(std::false_type{});
-        gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c);
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
-            raw[P - 1][i].pin();
-            up[i].pin();
+            for (int v = 0; v < V; ++v) h[v] = first[v];
         }
-        auto run = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
-            // the states of half a tile at a time: the first half's are computed twice
-            // (two operations each), and half of them in registers is enough
-            constexpr int HALF = GS_R / 2;
-            float first[V], before[HALF][V];
+        if (l.live) {
+            const float zero[V] = {};
+            for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t)
 #pragma unroll
-            for (int v = 0; v < V; ++v) first[v] = h[v];
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-                const bool in = FULL || t0 + i < l.len;
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
-            }
-#pragma unroll
-            for (int half = 1; half >= 0; --half) {
-#pragma unroll
-                for (int n = 0; n < HALF; ++n) {
-                    const int i = half * HALF + n;
-                    const bool in = FULL || t0 + i < l.len;
-                    raw[0][i].pin();
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        before[n][v] = h[v];
-                        h[v] = in ? fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]) : h[v];
-                    }
-                }
-#pragma unroll
-                for (int n = HALF - 1; n >= 0; --n) {
-                    const int i = half * HALF + n;
-                    const bool in = FULL || t0 + i < l.len;
-                    float out[P][V];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float x = raw[0][i].get(v), kk = k[i][v], hp = before[n][v];
-                        float g = up[i].get(v);
-                        if constexpr (P == 3) {
-                            const float z = raw[2][i].get(v);
-                            const float s = gs_sigmoid(z), zs = z * s;
-                            const float hn = fmaf(kk, x - hp, hp);
-                            out[2][v] = in ? g * hn * fmaf(zs, 1.f - s, s) : 0.f;
-                            g *= zs;
-                        }
-                        g += c[v];
-                        const float gk = g * kk;
-                        c[v] = in ? g - gk : c[v];
-                        out[0][v] = in ? gk : 0.f;
-                        out[1][v] = in ? (hp - x) * fmaf(-kk, gk, gk) : 0.f;
-                    }
-                    if (l.live && (FULL || t0 + i < a.T)) {
-#pragma unroll
-                        for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)(t0 + i) * P + q) * a.D, out[q]);
-                    }
-                    gs_fence<W>(i);
-                }
-#pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = first[v];
-            }
-        };
-        if (whole) run(std::true_type{});
-        else run(std::false_type{});
+                for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)t * P + q) * a.D, zero);
+        }
         if (l.live && a.dh0 != nullptr && tile == 0) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.dh0[(int64_t)l.b * a.D + l.d + v] = c[v];
