@@ -140,6 +140,8 @@ def weight_grad8(
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     O = dy2.shape[1]
     if dy2.is_cuda:
+        if dy2.dtype == torch.float16 and saved.dtype != torch.float16:
+            dy2 = dy2.float()  # the kept values are exact in float16 only if they came from it
         dw = torch.empty((O, F), dtype=dtype, device=dy2.device)
         db = torch.empty((O,), dtype=dtype, device=dy2.device) if bias else None
         ext().weight_grad8(dy2, saved.codes, saved.scales, dw, db)

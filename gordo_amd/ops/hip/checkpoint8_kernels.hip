@@ -11,7 +11,6 @@ namespace {
 typedef __bf16 c8_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 c8_f16x8 __attribute__((ext_vector_type(8)));
 typedef float c8_f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short c8_u16x8 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------------------
 // save8: a group of 32 is two values in each of 16 lanes. load8: the reverse.
@@ -48,14 +47,22 @@ __global__ __launch_bounds__(256) void c8_load(const signed char* codes, const u
 
 // ---------------------------------------------------------------------------
 // weight gradient: dW[o][f] = sum_n dy[n][o] * x8[n][f], db[o] = sum_n dy[n][o].
-// Both operands have the summed axis outermost, so tiles go to LDS transposed.
+//
+// Both operands have the summed axis outermost, while a matrix instruction wants
+// eight consecutive n of one o or f in a lane. The tiles go to LDS as they lie in
+// memory, and the transposing LDS read (ds_read_b64_tr_b16: 16 lanes read four rows
+// of 16 columns, each gets one column) turns them on the way to the registers.
+// Codes become 16-bit numbers between memory and LDS, exactly, so the product reads
+// one byte a value and nothing is restored in memory.
+//
 // 32-bit dy is taken as a sum of three bf16 numbers (8 + 8 + 8 bits: all of its
-// 24), one product each; x8 is exact in bf16 and in fp16.
+// 24), one product each; x8 is exact in bf16.
+//
+// Rows of a tile are cut into 32-byte chunks, and row k has its chunks permuted by
+// k & 3: the four rows of a transposing read lie in different banks.
 // ---------------------------------------------------------------------------
-#define WG_M 128
-#define WG_N 128
-#define WG_K 32
-#define WG_PITCH 40  // 16-bit elements of a tile row: 32 and a pad, rows stay 16-byte aligned
+#define WG_K 64  // rows of dy and x8 that are in LDS at a time
+#define WG_THREADS 512
 
 struct WgArgs {
     const void* dy;  // [N][O], rows at sdy
@@ -66,111 +73,234 @@ struct WgArgs {
     void* db;      // [O], or fp32 [splits][O], or null
     int64_t N, per;  // rows, and rows of one split
     int O, F, Fp;
-    int splits;
+    int tiles_f, tiles_o, splits;
 };
-
-// pieces of one dy value as 16-bit patterns
-__device__ __forceinline__ void wg_pieces(C8Bf16, unsigned short u, unsigned short* o) { o[0] = u; }
-__device__ __forceinline__ void wg_pieces(C8Fp16, unsigned short u, unsigned short* o) { o[0] = u; }
-__device__ __forceinline__ void wg_pieces(C8Fp32, float f, unsigned short* o) {
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        o[j] = C8Bf16::down(f);
-        f -= C8Bf16::up(o[j]);
-    }
-}
 
 template <class E>
 struct WgPieces { static const int n = 1; };
 template <>
 struct WgPieces<C8Fp32> { static const int n = 3; };
 
+__device__ __forceinline__ unsigned int wg_pair(unsigned short a, unsigned short b) { return (unsigned int)a | ((unsigned int)b << 16); }
+
+// place of 8 columns (16 bytes), number `c`, of row k in a tile with `pitch` bytes a row
+__device__ __forceinline__ int wg_at(int k, int c, int pitch) { return k * pitch + ((((c >> 1) ^ (k & 3)) << 5) | ((c & 1) << 4)); }
+
+typedef short wg_s16x4 __attribute__((ext_vector_type(4)));
+typedef short wg_s16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ wg_s16x4 wg_turn(const char* at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wg_s16x4*)at);
+}
+
 template <class E>
-__device__ __forceinline__ c8_f32x4 wg_mfma(c8_u16x8 a, c8_u16x8 b, c8_f32x4 c) {
-    union { c8_u16x8 u; c8_bf16x8 h; c8_f16x8 f; } x, y;
+__device__ __forceinline__ c8_f32x4 wg_mfma(wg_s16x8 a, wg_s16x8 b, c8_f32x4 c) {
+    union { wg_s16x8 u; c8_bf16x8 h; c8_f16x8 f; } x, y;
     x.u = a;
     y.u = b;
     if constexpr (std::is_same<E, C8Fp16>::value) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.f, y.f, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.h, y.h, c, 0, 0, 0);
 }
 
-// E: type of dy; G: type of the gradient; C: type that x8 is multiplied in
-template <class E, class G>
-__global__ __launch_bounds__(256) void c8_weight_grad(WgArgs a) {
-    typedef typename std::conditional<std::is_same<E, C8Fp16>::value, C8Fp16, C8Bf16>::type C;
-    const int NP = WgPieces<E>::n;
-    __shared__ __attribute__((aligned(16))) unsigned short A[WgPieces<E>::n][WG_M][WG_PITCH];
-    __shared__ __attribute__((aligned(16))) unsigned short B[WG_N][WG_PITCH];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    const int f0 = blockIdx.x * WG_N, o0 = blockIdx.y * WG_M;
-    const int64_t n0 = blockIdx.z * a.per, n1 = min(a.N, n0 + a.per);
-    const typename E::store* dy = (const typename E::store*)a.dy;
-    const int ng = a.Fp / C8_GROUP;
-    const int wm = (wid >> 1) * 64, wn = (wid & 1) * 64;
+// eight neighbouring values of a row of dy
+template <class E>
+struct WgEight {
+    typename E::store v[8];
+};
 
-    c8_f32x4 acc[4][4];
+template <class E, bool ALIGNED>
+__device__ __forceinline__ void wg_load(WgEight<E>& to, const typename E::store* row, int o, int O, bool in) {
+    if constexpr (ALIGNED) {
+        if (in && o < O) {
+            to = *(const WgEight<E>*)__builtin_assume_aligned(row + o, 16);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i) to.v[i] = 0;
+        }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = c8_f32x4{0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;  // of dy's column o0 + tid
+        for (int i = 0; i < 8; ++i) to.v[i] = in && o + i < O ? row[o + i] : (typename E::store)0;
+    }
+}
 
-    for (int64_t n = n0; n < n1; n += WG_K) {
-        __syncthreads();
-        for (int e = tid; e < WG_K * WG_M; e += 256) {
-            const int r = e / WG_M, c = e % WG_M;
-            unsigned short o[3] = {0, 0, 0};
-            if (n + r < n1 && o0 + c < a.O) wg_pieces(E{}, dy[(n + r) * a.sdy + o0 + c], o);
+// eight codes and their scale as 16-bit numbers
+template <class E>
+__device__ __forceinline__ uint4 wg_decode(uint2 codes, unsigned int scale) {
+    const float s = c8_step(scale), off = -128.f * s;
+    unsigned int out[4];
 #pragma unroll
-            for (int j = 0; j < NP; ++j) A[j][c][r] = o[j];
-        }
-        for (int e = tid; e < WG_K * WG_N; e += 256) {
-            const int r = e / WG_N, c = e % WG_N;
-            float v = 0.f;
-            if (n + r < n1 && f0 + c < a.F)
-                v = (float)a.codes[(n + r) * a.Fp + f0 + c] * c8_step(a.scales[(n + r) * ng + (f0 + c) / C8_GROUP]);
-            B[c][r] = C::down(v);
-        }
-        __syncthreads();
-        if (blockIdx.x == 0 && a.db != nullptr && tid < WG_M) {
-            for (int r = 0; r < WG_K; ++r) {
-                float v = 0.f;
-#pragma unroll
-                for (int j = 0; j < NP; ++j) v += C::up(A[j][tid][r]);
-                sum += v;
-            }
-        }
-        c8_u16x8 fb[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fb[j] = *(const c8_u16x8*)&B[wn + j * 16 + (lane & 15)][(lane >> 4) * 8];
-#pragma unroll
-        for (int q = 0; q < NP; ++q) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const c8_u16x8 fa = *(const c8_u16x8*)&A[q][wm + i * 16 + (lane & 15)][(lane >> 4) * 8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = wg_mfma<E>(fa, fb[j], acc[i][j]);
-            }
+    for (int h = 0; h < 2; ++h) {
+        const unsigned int w = (h == 0 ? codes.x : codes.y) ^ 0x80808080u;  // code + 128, unsigned
+        const float f0 = fmaf((float)(w & 0xff), s, off), f1 = fmaf((float)((w >> 8) & 0xff), s, off);
+        const float f2 = fmaf((float)((w >> 16) & 0xff), s, off), f3 = fmaf((float)(w >> 24), s, off);
+        if constexpr (std::is_same<E, C8Fp16>::value) {
+            out[2 * h] = wg_pair(C8Fp16::down(f0), C8Fp16::down(f1));
+            out[2 * h + 1] = wg_pair(C8Fp16::down(f2), C8Fp16::down(f3));
+        } else {  // exact: the upper halves are the numbers
+            out[2 * h] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
+            out[2 * h + 1] = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u);
         }
     }
-    // a lane holds rows (lane >> 4) * 4 + r of column lane & 15
-    const int64_t slab = (int64_t)blockIdx.z * a.O * a.F;
+    return uint4{out[0], out[1], out[2], out[3]};
+}
+
+// four neighbouring values, as one access where rows allow it
+template <class G>
+__device__ __forceinline__ void wg_store(typename G::store* to, c8_f32x4 v, int f, int F) {
+    if ((F & 3) == 0) {
+        struct alignas(sizeof(typename G::store) * 4) Four { typename G::store v[4]; };
+        *(Four*)to = Four{{G::down(v[0]), G::down(v[1]), G::down(v[2]), G::down(v[3])}};
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int r = 0; r < 4; ++r)
+            if (f + r < F) to[r] = G::down(v[r]);
+    }
+}
+
+// E: type of dy; G: type of the gradient. Eight waves, 2 along O and 4 along F.
+template <class E, class G, int BM, int BN, bool ALIGNED>
+__global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
+    constexpr int NP = WgPieces<E>::n;
+    constexpr int PA = BM * 2, PB = BN * 2;                    // bytes of a tile row
+    constexpr int SA = WG_K * PA, SB = WG_K * PB;              // bytes of a tile
+    constexpr int CA = BM / 8, CB = BN / 8;                    // eights of a tile row
+    constexpr int RA = WG_THREADS / CA, RB = WG_THREADS / CB;  // rows that the block takes at a time
+    constexpr int NA = WG_K / RA, NB = WG_K / RB;
+    constexpr int MI = BM / 32, NI = BN / 64;
+    __shared__ __attribute__((aligned(16))) char lds[2][NP * SA + SB];
+
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Blocks go to the eight XCDs in turn: neighbours in the order of the tiles, which
+    // share rows of dy or x8, are given to one XCD and its L2.
+    const int total = gridDim.x, each = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
+    const int place = xcd * each + min(xcd, rest) + (blockIdx.x >> 3);
+    const int tf = place % a.tiles_f, to = place / a.tiles_f % a.tiles_o, split = place / a.tiles_f / a.tiles_o;
+    const int f0 = tf * BN, o0 = to * BM;
+    const int64_t n0 = split * a.per, n1 = min(a.N, n0 + a.per);
+    const int ng = a.Fp / C8_GROUP;
+
+    const int ca = tid % CA, ra = tid / CA, cb = tid % CB, rb = tid / CB;
+    const typename E::store* dy = (const typename E::store*)a.dy;
+    WgEight<E> va[NA];
+    uint2 vb[NB];
+    unsigned int vs[NB];
+    auto load = [&](int64_t n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < NA; ++i) {
+            const int64_t row = n + ra + i * RA;
+            wg_load<E, ALIGNED>(va[i], dy + row * a.sdy, o0 + ca * 8, a.O, row < n1);
+        }
+        const int f = f0 + cb * 8;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int o = o0 + wm + i * 16 + (lane >> 4) * 4 + r, f = f0 + wn + j * 16 + (lane & 15);
-                if (o < a.O && f < a.F) {
-                    const int64_t at = (int64_t)o * a.F + f;
-                    if (a.splits > 1) ((float*)a.dw)[slab + at] = acc[i][j][r];
-                    else ((typename G::store*)a.dw)[at] = G::down(acc[i][j][r]);
+        for (int i = 0; i < NB; ++i) {
+            const int64_t row = n + rb + i * RB;
+            vb[i] = uint2{0u, 0u};
+            vs[i] = 127u;
+            if (row < n1 && f < a.Fp) {
+                vb[i] = *(const uint2*)(a.codes + row * a.Fp + f);
+                vs[i] = a.scales[row * ng + f / C8_GROUP];
+            }
+        }
+    };
+    const bool sums = tf == 0 && a.db != nullptr;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto put = [&](char* buf) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            char* at = buf + wg_at(ra + i * RA, ca, PA);
+            if constexpr (NP == 1) {
+                *(WgEight<E>*)at = va[i];
+            } else {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = E::up(va[i].v[e]);
+#pragma unroll
+                for (int q = 0; q < NP; ++q) {
+                    unsigned short h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        h[e] = C8Bf16::down(f[e]);
+                        f[e] -= C8Bf16::up(h[e]);
+                    }
+                    *(uint4*)(at + q * SA) = uint4{wg_pair(h[0], h[1]), wg_pair(h[2], h[3]), wg_pair(h[4], h[5]), wg_pair(h[6], h[7])};
                 }
             }
-    if (blockIdx.x == 0 && a.db != nullptr && tid < WG_M && o0 + tid < a.O) {
-        if (a.splits > 1) ((float*)a.db)[(int64_t)blockIdx.z * a.O + o0 + tid] = sum;
-        else ((typename G::store*)a.db)[o0 + tid] = G::down(sum);
+            if (sums) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += E::up(va[i].v[e]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) *(uint4*)(buf + NP * SA + wg_at(rb + i * RB, cb, PB)) = wg_decode<E>(vb[i], vs[i]);
+    };
+
+    c8_f32x4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = c8_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // a lane's part of a transposing read: row (lane >> 4) * 8 + (lane >> 2 & 3), 4 columns
+    const int row = (lane >> 4) * 8 + ((lane >> 2) & 3), sub = (lane & 3) * 8;
+    auto frag = [&](const char* tile, int pitch, int chunk, int k) {
+        const char* at = tile + (k + row) * pitch + ((chunk ^ (row & 3)) << 5) + sub;
+        const wg_s16x4 lo = wg_turn(at), hi = wg_turn(at + 4 * pitch);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    const int wm = (wid >> 2) * (BM / 2), wn = (wid & 3) * (BN / 4);
+    auto work = [&](const char* buf) {
+#pragma unroll
+        for (int k = 0; k < WG_K; k += 32) {
+            wg_s16x8 fb[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) fb[j] = frag(buf + NP * SA, PB, wn / 16 + j, k);
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const wg_s16x8 fa = frag(buf + q * SA, PA, wm / 16 + i, k);
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = wg_mfma<E>(fb[j], fa, acc[i][j]);
+                }
+        }
+    };
+
+    int buf = 0;
+    load(n0);
+    put(lds[0]);
+    __syncthreads();
+    for (int64_t n = n0; n < n1; n += WG_K) {
+        const bool more = n + WG_K < n1;
+        if (more) load(n + WG_K);
+        work(lds[buf]);
+        buf ^= 1;
+        if (more) put(lds[buf]);
+        __syncthreads();
+    }
+
+    // a lane holds four f, at (lane >> 4) * 4, of one o, lane & 15
+    const int64_t slab = (int64_t)split * a.O * a.F;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int o = o0 + wm + i * 16 + (lane & 15), f = f0 + wn + j * 16 + (lane >> 4) * 4;
+            if (o >= a.O || f >= a.F) continue;
+            const int64_t at = (int64_t)o * a.F + f;
+            if (a.splits > 1) wg_store<C8Fp32>((float*)a.dw + slab + at, acc[i][j], f, a.F);
+            else wg_store<G>((typename G::store*)a.dw + at, acc[i][j], f, a.F);
+        }
+    if (sums) {
+        float* part = (float*)lds;  // [RA][BM]
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[ra * BM + ca * 8 + e] = sum[e];
+        __syncthreads();
+        if (tid < BM && o0 + tid < a.O) {
+            float v = 0.f;
+            for (int r = 0; r < RA; ++r) v += part[r * BM + tid];
+            if (a.splits > 1) ((float*)a.db)[(int64_t)split * a.O + o0 + tid] = v;
+            else ((typename G::store*)a.db)[o0 + tid] = G::down(v);
+        }
     }
 }
 
@@ -251,7 +381,7 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     const int64_t N = dy.size(0), O = dy.size(1), F = dw.size(1), Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
     c8_check(codes, scales, N, F);
     TORCH_CHECK(codes.device() == dy.device(), "weight_grad8: dy and the codes are on different devices");
-    TORCH_CHECK(O > 0 && O <= INT_MAX - WG_M, "weight_grad8: O out of range");
+    TORCH_CHECK(O > 0 && O <= INT_MAX - 256, "weight_grad8: O out of range");
     if (db.has_value())
         TORCH_CHECK(db->device() == dy.device() && db->is_contiguous() && db->numel() == O && db->scalar_type() == dw.scalar_type(),
                     "weight_grad8: db must be contiguous [O] of the type of dw");
@@ -266,13 +396,20 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     a.O = (int)O;
     a.F = (int)F;
     a.Fp = (int)Fp;
-    const int64_t tf = (F + WG_N - 1) / WG_N, to = (O + WG_M - 1) / WG_M;
-    TORCH_CHECK(to <= 65535, "weight_grad8: O out of range");
-    // enough blocks for the chip, but at least 256 rows a split
-    int64_t splits = std::min<int64_t>(512 / (tf * to), (N + 255) / 256);
+    // Tiles of 256 x 256 read each operand least; 128 x 128 where those are too few, or
+    // three pieces of dy would not fit LDS.
+    const bool wide = dy.scalar_type() != at::kFloat && O > 128 && F > 128 && ((O + 255) / 256) * ((F + 255) / 256) * ((N + 511) / 512) >= 128;
+    const int64_t side = wide ? 256 : 128;
+    a.tiles_f = (int)((F + side - 1) / side);
+    a.tiles_o = (int)((O + side - 1) / side);
+    const int64_t tiles = (int64_t)a.tiles_f * a.tiles_o;
+    // blocks for the chip (one a CU, or two of the small ones), but at least 256 rows a split
+    int64_t splits = std::min<int64_t>((wide ? 256 : 512) / tiles, (N + 255) / 256);
     splits = std::max<int64_t>(1, splits);
     a.per = (((N + splits - 1) / splits) + WG_K - 1) / WG_K * WG_K;
     a.splits = (int)(a.per > 0 ? std::max<int64_t>(1, (N + a.per - 1) / a.per) : 1);
+    TORCH_CHECK(tiles * a.splits <= INT_MAX, "weight_grad8: sizes out of range");
+    const bool aligned = O % 8 == 0 && a.sdy % 8 == 0 && (uintptr_t)a.dy % 16 == 0;
     torch::Tensor part, part_b;
     const bool join = a.splits > 1;
     if (join) {
@@ -287,12 +424,17 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
         a.dw = dw.data_ptr();
         a.db = db.has_value() ? db->data_ptr() : nullptr;
     }
-    const dim3 grid((unsigned)tf, (unsigned)to, (unsigned)a.splits);
+    const dim3 grid((unsigned)(tiles * a.splits));
     c8_type(dy.scalar_type(), "weight_grad8: dy", [&](auto e) {
         c8_type(dw.scalar_type(), "weight_grad8: dw", [&](auto g) {
             typedef decltype(e) E;
             typedef decltype(g) G;
-            hipLaunchKernelGGL((c8_weight_grad<E, G>), dim3(grid), dim3(256), 0, stream, a);
+            if constexpr (WgPieces<E>::n == 1) {
+                if (wide && aligned) hipLaunchKernelGGL((c8_weight_grad<E, G, 256, 256, true>), grid, dim3(WG_THREADS), 0, stream, a);
+                else if (wide) hipLaunchKernelGGL((c8_weight_grad<E, G, 256, 256, false>), grid, dim3(WG_THREADS), 0, stream, a);
+            }
+            if (!wide && aligned) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, true>), grid, dim3(WG_THREADS), 0, stream, a);
+            else if (!wide) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, false>), grid, dim3(WG_THREADS), 0, stream, a);
             if (join) {
                 hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(O * F)), dim3(256), 0, stream, (const float*)part.data_ptr(), (typename G::store*)dw.data_ptr(), O * F, a.splits);
                 if (db.has_value())

@@ -177,6 +177,25 @@ def test_weight_gradient(device, dtype, N, F, O):
     check_weight_grad(dy, values(N, F, dtype, device).clamp(-100, 100), dtype)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("N,F,O", [(12000, 300, 520), (12001, 301, 517), (11000, 512, 512), (600, 1500, 2100)])
+def test_weight_gradient_of_wide_layers(dtype, N, F, O):
+    g = torch.Generator().manual_seed(N)
+    dy = torch.randn(N, O, generator=g).to(dtype).cuda()
+    check_weight_grad(dy, torch.randn(N, F, generator=g).to(dtype).cuda(), dtype)
+    check_weight_grad(dy, torch.randn(N, F, generator=g).to(dtype).cuda(), torch.float32, bias=False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_weight_gradient_of_values_beyond_float16(device):
+    """dy in float16 beside an input that was kept from float32."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(50, 40, generator=g).to(device) * 2.0**40
+    dy = torch.randn(50, 24, generator=g).to(torch.float16).to(device)
+    check_weight_grad(dy, x, torch.float32)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("of_dy", DTYPES, ids=str)
 @pytest.mark.parametrize("to", DTYPES, ids=str)
