@@ -59,7 +59,8 @@ __global__ __launch_bounds__(256) void c8_load(const signed char* codes, const u
 // 24), one product each; x8 is exact in bf16.
 //
 // Rows of a tile are cut into 32-byte chunks, and row k has its chunks permuted by
-// k & 3: the four rows of a transposing read lie in different banks.
+// (k & 3) + 4 * (k >> 3 & 1): the eight rows that half a wave's transposing read
+// takes (0..3 and 8..11 of a fragment) lie in different banks, all 64 of them.
 // ---------------------------------------------------------------------------
 #define WG_K 64  // rows of dy and x8 that are in LDS at a time
 #define WG_THREADS 512
@@ -83,8 +84,10 @@ struct WgPieces<C8Fp32> { static const int n = 3; };
 
 __device__ __forceinline__ unsigned int wg_pair(unsigned short a, unsigned short b) { return (unsigned int)a | ((unsigned int)b << 16); }
 
+__device__ __forceinline__ int wg_mix(int k) { return (k & 3) | ((k >> 1) & 4); }
+
 // place of 8 columns (16 bytes), number `c`, of row k in a tile with `pitch` bytes a row
-__device__ __forceinline__ int wg_at(int k, int c, int pitch) { return k * pitch + ((((c >> 1) ^ (k & 3)) << 5) | ((c & 1) << 4)); }
+__device__ __forceinline__ int wg_at(int k, int c, int pitch) { return k * pitch + ((((c >> 1) ^ wg_mix(k)) << 5) | ((c & 1) << 4)); }
 
 typedef short wg_s16x4 __attribute__((ext_vector_type(4)));
 typedef short wg_s16x8 __attribute__((ext_vector_type(8)));
@@ -108,20 +111,16 @@ struct WgEight {
     typename E::store v[8];
 };
 
-template <class E, bool ALIGNED>
-__device__ __forceinline__ void wg_load(WgEight<E>& to, const typename E::store* row, int o, int O, bool in) {
-    if constexpr (ALIGNED) {
-        if (in && o < O) {
-            to = *(const WgEight<E>*)__builtin_assume_aligned(row + o, 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) to.v[i] = 0;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) to.v[i] = in && o + i < O ? row[o + i] : (typename E::store)0;
-    }
+// A buffer of the rows that are left, from this one on: what lies behind them reads as 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t wg_rows(const void* at, int64_t left, int64_t row_bytes) {
+    const int64_t bytes = left > 0 ? left * row_bytes : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes < 0x7fffffff ? (int)bytes : 0x7fffffff, 0x00027000);
 }
+
+#define WG_OUT 0x7ffffff0  // an offset behind every buffer
+
+typedef unsigned int wg_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int wg_u32x2 __attribute__((ext_vector_type(2)));
 
 // eight codes and their scale as 16-bit numbers
 template <class E>
@@ -181,25 +180,41 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
 
     const int ca = tid % CA, ra = tid / CA, cb = tid % CB, rb = tid / CB;
     const typename E::store* dy = (const typename E::store*)a.dy;
+    constexpr int ES = sizeof(typename E::store);
+    // ALIGNED: rows of dy are whole 16-byte words, so are a lane's eight values
+    const int oa = o0 + ca * 8 < a.O ? (ra * (int)a.sdy + o0 + ca * 8) * ES : WG_OUT;
+    const int fb8 = f0 + cb * 8;
+    const int ob = fb8 < a.Fp ? rb * a.Fp + fb8 : WG_OUT, os = fb8 < a.Fp ? rb * ng + fb8 / C8_GROUP : WG_OUT;
     WgEight<E> va[NA];
     uint2 vb[NB];
     unsigned int vs[NB];
     auto load = [&](int64_t n) {
+        if constexpr (ALIGNED) {
+            const auto rows = wg_rows(dy + n * a.sdy, n1 - n, a.sdy * ES);
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int64_t row = n + ra + i * RA;
-            wg_load<E, ALIGNED>(va[i], dy + row * a.sdy, o0 + ca * 8, a.O, row < n1);
+            for (int i = 0; i < NA; ++i) {
+                const int at = oa + i * RA * (int)a.sdy * ES;
+                wg_u32x4* to = (wg_u32x4*)&va[i];
+#pragma unroll
+                for (int h = 0; h < ES / 2; ++h) to[h] = __builtin_amdgcn_raw_buffer_load_b128(rows, oa == WG_OUT ? WG_OUT : at + h * 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int64_t row = n + ra + i * RA;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int o = o0 + ca * 8 + e;
+                    va[i].v[e] = row < n1 && o < a.O ? dy[row * a.sdy + o] : (typename E::store)0;
+                }
+            }
         }
-        const int f = f0 + cb * 8;
+        const auto codes = wg_rows(a.codes + n * a.Fp, n1 - n, a.Fp), scales = wg_rows(a.scales + n * ng, n1 - n, ng);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int64_t row = n + rb + i * RB;
-            vb[i] = uint2{0u, 0u};
-            vs[i] = 127u;
-            if (row < n1 && f < a.Fp) {
-                vb[i] = *(const uint2*)(a.codes + row * a.Fp + f);
-                vs[i] = a.scales[row * ng + f / C8_GROUP];
-            }
+            const wg_u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(codes, ob == WG_OUT ? WG_OUT : ob + i * RB * a.Fp, 0, 0);
+            vb[i] = uint2{w[0], w[1]};
+            vs[i] = __builtin_amdgcn_raw_buffer_load_b8(scales, os == WG_OUT ? WG_OUT : os + i * RB * ng, 0, 0);
         }
     };
     const bool sums = tf == 0 && a.db != nullptr;
@@ -243,38 +258,55 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     // a lane's part of a transposing read: row (lane >> 4) * 8 + (lane >> 2 & 3), 4 columns
     const int row = (lane >> 4) * 8 + ((lane >> 2) & 3), sub = (lane & 3) * 8;
     auto frag = [&](const char* tile, int pitch, int chunk, int k) {
-        const char* at = tile + (k + row) * pitch + ((chunk ^ (row & 3)) << 5) + sub;
+        const char* at = tile + (k + row) * pitch + ((chunk ^ wg_mix(row)) << 5) + sub;
         const wg_s16x4 lo = wg_turn(at), hi = wg_turn(at + 4 * pitch);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     const int wm = (wid >> 2) * (BM / 2), wn = (wid & 3) * (BN / 4);
+    // One step is a fragment of dy against all of x8's. Fragments are read two steps
+    // before they are used, and the order is held: left alone, the compiler reads one,
+    // waits for it, and the matrix unit waits too.
     auto work = [&](const char* buf) {
+        constexpr int S = MI * NP, ALL = 2 * S;
+        wg_s16x8 fa[3], fb[2][NI];
+        auto read_a = [&](int s) { return frag(buf + (s % S / MI) * SA, PA, wm / 16 + s % MI, s / S * 32); };
+        auto read_b = [&](int j, int k) { return frag(buf + NP * SA, PB, wn / 16 + j, k); };
 #pragma unroll
-        for (int k = 0; k < WG_K; k += 32) {
-            wg_s16x8 fb[NI];
+        for (int j = 0; j < NI; ++j) fb[0][j] = read_b(j, 0);
+        fa[0] = read_a(0);
+        fa[1] = read_a(1);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) fb[j] = frag(buf + NP * SA, PB, wn / 16 + j, k);
+        for (int s = 0; s < ALL; ++s) {
+            if (s + 2 < ALL) fa[(s + 2) % 3] = read_a(s + 2);
+            if (s < NI) fb[1][s] = read_b(s, 32);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int q = 0; q < NP; ++q)
-#pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    const wg_s16x8 fa = frag(buf + q * SA, PA, wm / 16 + i, k);
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = wg_mfma<E>(fb[j], fa, acc[i][j]);
-                }
+            for (int j = 0; j < NI; ++j) acc[s % MI][j] = wg_mfma<E>(fb[s / S][j], fa[s % 3], acc[s % MI][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
+    // Two waves share a SIMD, wid and wid + 4. One decodes the next tile before its
+    // products and the other after them, so that one's conversions and LDS writes run
+    // beside the other's matrix instructions. Loads are a whole tile ahead either way.
+    const bool early = wid < 4;
     int buf = 0;
     load(n0);
     put(lds[0]);
+    load(n0 + WG_K);  // rows behind n1 are zeros
     __syncthreads();
     for (int64_t n = n0; n < n1; n += WG_K) {
         const bool more = n + WG_K < n1;
-        if (more) load(n + WG_K);
+        if (early && more) {
+            put(lds[buf ^ 1]);
+            load(n + 2 * WG_K);
+        }
         work(lds[buf]);
         buf ^= 1;
-        if (more) put(lds[buf]);
+        if (!early && more) {
+            put(lds[buf]);
+            load(n + 2 * WG_K);
+        }
         __syncthreads();
     }
 
@@ -381,7 +413,7 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     const int64_t N = dy.size(0), O = dy.size(1), F = dw.size(1), Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
     c8_check(codes, scales, N, F);
     TORCH_CHECK(codes.device() == dy.device(), "weight_grad8: dy and the codes are on different devices");
-    TORCH_CHECK(O > 0 && O <= INT_MAX - 256, "weight_grad8: O out of range");
+    TORCH_CHECK(O > 0 && O <= (1 << 24) && F <= (1 << 24), "weight_grad8: O or F out of range");
     if (db.has_value())
         TORCH_CHECK(db->device() == dy.device() && db->is_contiguous() && db->numel() == O && db->scalar_type() == dw.scalar_type(),
                     "weight_grad8: db must be contiguous [O] of the type of dw");
@@ -409,7 +441,8 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     a.per = (((N + splits - 1) / splits) + WG_K - 1) / WG_K * WG_K;
     a.splits = (int)(a.per > 0 ? std::max<int64_t>(1, (N + a.per - 1) / a.per) : 1);
     TORCH_CHECK(tiles * a.splits <= INT_MAX, "weight_grad8: sizes out of range");
-    const bool aligned = O % 8 == 0 && a.sdy % 8 == 0 && (uintptr_t)a.dy % 16 == 0;
+    // whole 16-byte words, and a tile's rows within 31-bit offsets
+    const bool aligned = O % 8 == 0 && a.sdy % 8 == 0 && a.sdy >= O && a.sdy <= (1 << 22) && (uintptr_t)a.dy % 16 == 0;
     torch::Tensor part, part_b;
     const bool join = a.splits > 1;
     if (join) {
