@@ -13,6 +13,7 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #define C8_GROUP 32
 
@@ -73,13 +74,27 @@ __device__ __forceinline__ unsigned int c8_code_byte(float v, float inv) {
     return __float_as_uint(q) & 0xffu;
 }
 
-// max over 16 lanes of a row (DPP: no LDS pass)
-__device__ __forceinline__ unsigned int c8_max16(unsigned int m) {
+// f(integral_constant 0 .. N-1): for where an instruction wants a constant
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void c8_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        c8_for<N, I + 1>(f);
+    }
+}
+
+// max over 4 and over 16 neighbouring lanes (DPP: no LDS pass)
+__device__ __forceinline__ unsigned int c8_max4(unsigned int m) {
     unsigned int o;
     o = (unsigned int)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true);   // quad_perm 1,0,3,2
     m = m > o ? m : o;
     o = (unsigned int)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true);   // quad_perm 2,3,0,1
-    m = m > o ? m : o;
+    return m > o ? m : o;
+}
+
+__device__ __forceinline__ unsigned int c8_max16(unsigned int m) {
+    unsigned int o;
+    m = c8_max4(m);
     o = (unsigned int)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true);  // row_half_mirror
     m = m > o ? m : o;
     o = (unsigned int)__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xF, 0xF, true);  // row_mirror

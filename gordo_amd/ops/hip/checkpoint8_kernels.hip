@@ -13,35 +13,93 @@ typedef _Float16 c8_f16x8 __attribute__((ext_vector_type(8)));
 typedef float c8_f32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
-// save8: a group of 32 is two values in each of 16 lanes. load8: the reverse.
+// save8: a group of 32 is eight values in each of four lanes, so that a lane reads 16
+// or 32 bytes and writes 8; a lane takes WORK such eights, all loads before the first
+// use. load8: the reverse.
 // ---------------------------------------------------------------------------
+#define C8_WORK 4
+
 template <class E>
+struct alignas(16) C8Eight {
+    typename E::store v[8];
+};
+
+// VEC: rows start at 16-byte words and F is a multiple of 8
+template <class E, bool VEC>
 __global__ __launch_bounds__(256) void c8_save(const typename E::store* x, int64_t sx, signed char* codes,
                                                unsigned char* scales, int64_t N, int F, int Fp) {
-    const int64_t ng = Fp / C8_GROUP, all = N * ng * 16;
-    const int64_t step = (int64_t)gridDim.x * 256;
-    // `all` is a multiple of 16: the lanes of a group stay together
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
-        const int64_t row = i / (ng * 16);
-        const int col = (int)(i - row * ng * 16) * 2;
-        const float a = col < F ? E::up(x[row * sx + col]) : 0.f;
-        const float b = col + 1 < F ? E::up(x[row * sx + col + 1]) : 0.f;
-        const unsigned int s = c8_scale(c8_max16(max(c8_mag(a), c8_mag(b))));
+    // eights of the padded rows; a multiple of 4, so the lanes of a group stay together
+    const unsigned int each = Fp / 8;
+    const int64_t all = N * each, from = (int64_t)blockIdx.x * 256 * C8_WORK + threadIdx.x;
+    C8Eight<E> v[C8_WORK];
+    int64_t row[C8_WORK];
+    int col[C8_WORK];
+#pragma unroll
+    for (int k = 0; k < C8_WORK; ++k) {
+        const int64_t i = from + k * 256;
+        row[k] = i < all ? i / each : 0;
+        col[k] = i < all ? (int)(i - row[k] * each) * 8 : 0;
+        const typename E::store* at = x + row[k] * sx + col[k];
+        if constexpr (VEC) {
+            if (i < all && col[k] < F) v[k] = *(const C8Eight<E>*)at;
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k].v[e] = 0;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k].v[e] = i < all && col[k] + e < F ? at[e] : (typename E::store)0;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < C8_WORK; ++k) {
+        const int64_t i = from + k * 256;
+        unsigned int top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, c8_mag(E::up(v[k].v[e])));
+        const unsigned int s = c8_scale(c8_max4(top));
         const float inv = c8_inv(s);
-        *(unsigned short*)(codes + row * Fp + col) = (unsigned short)(c8_code_byte(a, inv) | (c8_code_byte(b, inv) << 8));
-        if (col % C8_GROUP == 0) scales[row * ng + col / C8_GROUP] = (unsigned char)s;
+        unsigned int w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = c8_code_byte(E::up(v[k].v[e]), inv);
+        if (i < all) {
+            *(uint2*)(codes + row[k] * Fp + col[k]) = uint2{w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24};
+            if (col[k] % C8_GROUP == 0) scales[row[k] * (Fp / C8_GROUP) + col[k] / C8_GROUP] = (unsigned char)s;
+        }
     }
 }
 
-template <class E>
+template <class E, bool VEC>
 __global__ __launch_bounds__(256) void c8_load(const signed char* codes, const unsigned char* scales,
                                                typename E::store* x, int64_t N, int F, int Fp) {
-    const int64_t ng = Fp / C8_GROUP, all = N * F;
-    const int64_t step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
-        const int64_t row = i / F;
-        const int col = (int)(i - row * F);
-        x[i] = E::down((float)codes[row * Fp + col] * c8_step(scales[row * ng + col / C8_GROUP]));
+    const unsigned int each = Fp / 8;
+    const int64_t all = N * each, from = (int64_t)blockIdx.x * 256 * C8_WORK + threadIdx.x;
+    uint2 c[C8_WORK];
+    unsigned int s[C8_WORK];
+    int64_t row[C8_WORK];
+    int col[C8_WORK];
+#pragma unroll
+    for (int k = 0; k < C8_WORK; ++k) {
+        const int64_t i = from + k * 256;
+        row[k] = i < all ? i / each : 0;
+        col[k] = i < all ? (int)(i - row[k] * each) * 8 : 0;
+        c[k] = *(const uint2*)(codes + row[k] * Fp + col[k]);
+        s[k] = scales[row[k] * (Fp / C8_GROUP) + col[k] / C8_GROUP];
+    }
+#pragma unroll
+    for (int k = 0; k < C8_WORK; ++k) {
+        if (from + k * 256 >= all || col[k] >= F) continue;
+        const float step = c8_step(s[k]);
+        C8Eight<E> v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = E::down((float)(signed char)((e < 4 ? c[k].x : c[k].y) >> (e % 4 * 8)) * step);
+        typename E::store* at = x + row[k] * F + col[k];
+        if constexpr (VEC) {
+            *(C8Eight<E>*)at = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col[k] + e < F) at[e] = v.v[e];
+        }
     }
 }
 
@@ -70,8 +128,8 @@ struct WgArgs {
     int64_t sdy;
     const signed char* codes;
     const unsigned char* scales;
-    void* dw;      // [O][F] in the output type, or fp32 [splits][O][F]
-    void* db;      // [O], or fp32 [splits][O], or null
+    void* dw;      // [O][F] in the output type, or fp32 [splits][O][Fq], Fq = F rounded up to 4
+    void* db;      // [O], or fp32 [splits][tiles_f][O rounded up to 4], or null
     int64_t N, per;  // rows, and rows of one split
     int O, F, Fp;
     int tiles_f, tiles_o, splits;
@@ -159,6 +217,7 @@ __device__ __forceinline__ void wg_store(typename G::store* to, c8_f32x4 v, int 
 // E: type of dy; G: type of the gradient. Eight waves, 2 along O and 4 along F.
 template <class E, class G, int BM, int BN, bool ALIGNED>
 __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
+    typedef typename std::conditional<std::is_same<E, C8Fp16>::value, C8Fp16, C8Bf16>::type C;  // type of the products
     constexpr int NP = WgPieces<E>::n;
     constexpr int PA = BM * 2, PB = BN * 2;                    // bytes of a tile row
     constexpr int SA = WG_K * PA, SB = WG_K * PB;              // bytes of a tile
@@ -184,69 +243,60 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     // ALIGNED: rows of dy are whole 16-byte words, so are a lane's eight values
     const int oa = o0 + ca * 8 < a.O ? (ra * (int)a.sdy + o0 + ca * 8) * ES : WG_OUT;
     const int fb8 = f0 + cb * 8;
-    const int ob = fb8 < a.Fp ? rb * a.Fp + fb8 : WG_OUT, os = fb8 < a.Fp ? rb * ng + fb8 / C8_GROUP : WG_OUT;
+    const int ob = fb8 < a.Fp ? rb * a.Fp + fb8 : WG_OUT;
+    // the four lanes of a quad have one group of 32 codes in each of their NB rows: lane i
+    // loads the scale of row i, and the others get it from there
+    static_assert(NB <= 4, "a scale for each lane of a quad");
+    const int os = fb8 < a.Fp ? (rb + (tid % NB) * RB) * ng + fb8 / C8_GROUP : WG_OUT;
     WgEight<E> va[NA];
     uint2 vb[NB];
-    unsigned int vs[NB];
-    auto load = [&](int64_t n) {
+    int vs;
+    auto load_a = [&](int i, int64_t n) {
         if constexpr (ALIGNED) {
             const auto rows = wg_rows(dy + n * a.sdy, n1 - n, a.sdy * ES);
+            const int at = oa + i * RA * (int)a.sdy * ES;
+            wg_u32x4* to = (wg_u32x4*)&va[i];
 #pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                const int at = oa + i * RA * (int)a.sdy * ES;
-                wg_u32x4* to = (wg_u32x4*)&va[i];
-#pragma unroll
-                for (int h = 0; h < ES / 2; ++h) to[h] = __builtin_amdgcn_raw_buffer_load_b128(rows, oa == WG_OUT ? WG_OUT : at + h * 16, 0, 0);
-            }
+            for (int h = 0; h < ES / 2; ++h) to[h] = __builtin_amdgcn_raw_buffer_load_b128(rows, oa == WG_OUT ? WG_OUT : at + h * 16, 0, 0);
         } else {
+            const int64_t row = n + ra + i * RA;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                const int64_t row = n + ra + i * RA;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int o = o0 + ca * 8 + e;
-                    va[i].v[e] = row < n1 && o < a.O ? dy[row * a.sdy + o] : (typename E::store)0;
-                }
+            for (int e = 0; e < 8; ++e) {
+                const int o = o0 + ca * 8 + e;
+                va[i].v[e] = row < n1 && o < a.O ? dy[row * a.sdy + o] : (typename E::store)0;
             }
-        }
-        const auto codes = wg_rows(a.codes + n * a.Fp, n1 - n, a.Fp), scales = wg_rows(a.scales + n * ng, n1 - n, ng);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const wg_u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(codes, ob == WG_OUT ? WG_OUT : ob + i * RB * a.Fp, 0, 0);
-            vb[i] = uint2{w[0], w[1]};
-            vs[i] = __builtin_amdgcn_raw_buffer_load_b8(scales, os == WG_OUT ? WG_OUT : os + i * RB * ng, 0, 0);
         }
     };
-    const bool sums = tf == 0 && a.db != nullptr;
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    auto put = [&](char* buf) {
+    auto load_b = [&](int i, int64_t n) {
+        const auto codes = wg_rows(a.codes + n * a.Fp, n1 - n, a.Fp);
+        const wg_u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(codes, ob == WG_OUT ? WG_OUT : ob + i * RB * a.Fp, 0, 0);
+        vb[i] = uint2{w[0], w[1]};
+        if (i == NB - 1) vs = __builtin_amdgcn_raw_buffer_load_b8(wg_rows(a.scales + n * ng, n1 - n, ng), os, 0, 0);
+    };
+    auto put_a = [&](int i, char* buf) {
+        char* at = buf + wg_at(ra + i * RA, ca, PA);
+        if constexpr (NP == 1) {
+            *(WgEight<E>*)at = va[i];
+        } else {
+            float f[8];
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            char* at = buf + wg_at(ra + i * RA, ca, PA);
-            if constexpr (NP == 1) {
-                *(WgEight<E>*)at = va[i];
-            } else {
-                float f[8];
+            for (int e = 0; e < 8; ++e) f[e] = E::up(va[i].v[e]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = E::up(va[i].v[e]);
+            for (int q = 0; q < NP; ++q) {
+                unsigned short h[8];
 #pragma unroll
-                for (int q = 0; q < NP; ++q) {
-                    unsigned short h[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        h[e] = C8Bf16::down(f[e]);
-                        f[e] -= C8Bf16::up(h[e]);
-                    }
-                    *(uint4*)(at + q * SA) = uint4{wg_pair(h[0], h[1]), wg_pair(h[2], h[3]), wg_pair(h[4], h[5]), wg_pair(h[6], h[7])};
+                for (int e = 0; e < 8; ++e) {
+                    h[e] = C8Bf16::down(f[e]);
+                    f[e] -= C8Bf16::up(h[e]);
                 }
-            }
-            if (sums) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] += E::up(va[i].v[e]);
+                *(uint4*)(at + q * SA) = uint4{wg_pair(h[0], h[1]), wg_pair(h[2], h[3]), wg_pair(h[4], h[5]), wg_pair(h[6], h[7])};
             }
         }
-#pragma unroll
-        for (int i = 0; i < NB; ++i) *(uint4*)(buf + NP * SA + wg_at(rb + i * RB, cb, PB)) = wg_decode<E>(vb[i], vs[i]);
+    };
+    auto put_b = [&](auto piece, char* buf) {
+        constexpr int i = decltype(piece)::value;
+        const int scale = __builtin_amdgcn_mov_dpp(vs, i * 0x55, 0xF, 0xF, true);  // quad_perm: lane i's to all four
+        *(uint4*)(buf + NP * SA + wg_at(rb + i * RB, cb, PB)) = wg_decode<E>(vb[i], scale);
     };
 
     c8_f32x4 acc[MI][NI];
@@ -264,10 +314,12 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     };
     const int wm = (wid >> 2) * (BM / 2), wn = (wid & 3) * (BN / 4);
     // One step is a fragment of dy against all of x8's. Fragments are read two steps
-    // before they are used, and the order is held: left alone, the compiler reads one,
-    // waits for it, and the matrix unit waits too.
-    auto work = [&](const char* buf) {
-        constexpr int S = MI * NP, ALL = 2 * S;
+    // before they are used. Between the steps the next tile is brought to LDS piece by
+    // piece and the loads of the one after it go out, so that conversions, LDS writes
+    // and loads run beside the matrix instructions. The order is held: left alone, the
+    // compiler reads a fragment, waits for it, and the matrix unit waits too.
+    auto tile = [&](const char* buf, char* next, int64_t n) {
+        constexpr int S = MI * NP, ALL = 2 * S, PIECES = NA + NB;
         wg_s16x8 fa[3], fb[2][NI];
         auto read_a = [&](int s) { return frag(buf + (s % S / MI) * SA, PA, wm / 16 + s % MI, s / S * 32); };
         auto read_b = [&](int j, int k) { return frag(buf + NP * SA, PB, wn / 16 + j, k); };
@@ -275,74 +327,109 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
         for (int j = 0; j < NI; ++j) fb[0][j] = read_b(j, 0);
         fa[0] = read_a(0);
         fa[1] = read_a(1);
-#pragma unroll
-        for (int s = 0; s < ALL; ++s) {
+        c8_for<ALL>([&](auto step) {
+            constexpr int s = decltype(step)::value;
             if (s + 2 < ALL) fa[(s + 2) % 3] = read_a(s + 2);
             if (s < NI) fb[1][s] = read_b(s, 32);
             __builtin_amdgcn_sched_barrier(0);
+            constexpr int from = s * PIECES / ALL, upto = (s + 1) * PIECES / ALL;
+            c8_for<upto - from>([&](auto k) {
+                constexpr int piece = from + decltype(k)::value;
+                if constexpr (piece < NA) {
+                    put_a(piece, next);
+                    load_a(piece, n + 2 * WG_K);
+                } else {
+                    put_b(std::integral_constant<int, piece - NA>{}, next);
+                    load_b(piece - NA, n + 2 * WG_K);
+                }
+            });
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[s % MI][j] = wg_mfma<E>(fb[s / S][j], fa[s % 3], acc[s % MI][j]);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction,
+                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // eight vector ones
+            }
             __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // dy's column sums, from LDS: the blocks of one o take the tiles in turn, so that none
+    // has more to do than the others. A thread has a column and a part of its rows.
+    constexpr int RS = WG_K * BM / WG_THREADS;
+    float sum = 0.f;
+    auto add = [&](const char* buf) {
+        const int c = tid % BM, r0 = tid / BM * RS;
+#pragma unroll 8
+        for (int r = r0; r < r0 + RS; ++r) {
+            const char* at = buf + wg_at(r, c >> 3, PA) + (c & 7) * 2;
+            float v = 0.f;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) v += C::up(*(const unsigned short*)(at + q * SA));  // exact
+            sum += v;
         }
     };
 
-    // Two waves share a SIMD, wid and wid + 4. One decodes the next tile before its
-    // products and the other after them, so that one's conversions and LDS writes run
-    // beside the other's matrix instructions. Loads are a whole tile ahead either way.
-    const bool early = wid < 4;
-    int buf = 0;
-    load(n0);
-    put(lds[0]);
-    load(n0 + WG_K);  // rows behind n1 are zeros
+    // behind n1 there are zeros: the last tiles need no case of their own
+#pragma unroll
+    for (int i = 0; i < NA; ++i) load_a(i, n0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) load_b(i, n0);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        put_a(i, lds[0]);
+        load_a(i, n0 + WG_K);
+    }
+    c8_for<NB>([&](auto i) {
+        put_b(i, lds[0]);
+        load_b(decltype(i)::value, n0 + WG_K);
+    });
     __syncthreads();
+    int buf = 0, turn = 0;
     for (int64_t n = n0; n < n1; n += WG_K) {
-        const bool more = n + WG_K < n1;
-        if (early && more) {
-            put(lds[buf ^ 1]);
-            load(n + 2 * WG_K);
-        }
-        work(lds[buf]);
+        if (a.db != nullptr && turn == tf) add(lds[buf]);
+        turn = turn + 1 == a.tiles_f ? 0 : turn + 1;
+        tile(lds[buf], lds[buf ^ 1], n);
         buf ^= 1;
-        if (!early && more) {
-            put(lds[buf]);
-            load(n + 2 * WG_K);
-        }
         __syncthreads();
     }
 
     // a lane holds four f, at (lane >> 4) * 4, of one o, lane & 15
-    const int64_t slab = (int64_t)split * a.O * a.F;
+    const int Fq = (a.F + 3) & ~3;
+    const int64_t slab = (int64_t)split * a.O * Fq;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             const int o = o0 + wm + i * 16 + (lane & 15), f = f0 + wn + j * 16 + (lane >> 4) * 4;
             if (o >= a.O || f >= a.F) continue;
-            const int64_t at = (int64_t)o * a.F + f;
-            if (a.splits > 1) wg_store<C8Fp32>((float*)a.dw + slab + at, acc[i][j], f, a.F);
-            else wg_store<G>((typename G::store*)a.dw + at, acc[i][j], f, a.F);
+            if (a.splits > 1) wg_store<C8Fp32>((float*)a.dw + slab + (int64_t)o * Fq + f, acc[i][j], f, Fq);
+            else wg_store<G>((typename G::store*)a.dw + (int64_t)o * a.F + f, acc[i][j], f, a.F);
         }
-    if (sums) {
-        float* part = (float*)lds;  // [RA][BM]
-#pragma unroll
-        for (int e = 0; e < 8; ++e) part[ra * BM + ca * 8 + e] = sum[e];
+    if (a.db != nullptr) {
+        float* part = (float*)lds;  // [WG_THREADS / BM][BM]
+        part[tid] = sum;
         __syncthreads();
         if (tid < BM && o0 + tid < a.O) {
             float v = 0.f;
-            for (int r = 0; r < RA; ++r) v += part[r * BM + tid];
-            if (a.splits > 1) ((float*)a.db)[(int64_t)split * a.O + o0 + tid] = v;
+#pragma unroll
+            for (int r = 0; r < WG_THREADS / BM; ++r) v += part[r * BM + tid];
+            if (a.splits * a.tiles_f > 1) ((float*)a.db)[((int64_t)split * a.tiles_f + tf) * ((a.O + 3) & ~3) + o0 + tid] = v;
             else ((typename G::store*)a.db)[o0 + tid] = G::down(v);
         }
     }
 }
 
-// sums the splits in their order
+// Sums the splits in their order: [splits][rows][pitch] to [rows][F], four values a lane.
 template <class G>
-__global__ __launch_bounds__(256) void c8_join(const float* part, typename G::store* out, int64_t n, int splits) {
+__global__ __launch_bounds__(256) void c8_join(const float* part, typename G::store* out, int64_t rows, int F, int pitch, int splits) {
+    const int64_t fours = pitch / 4, n = rows * fours;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += part[s * n + i];
-        out[i] = G::down(v);
+        const int64_t r = i / fours;
+        const int f = (int)(i - r * fours) * 4;
+        c8_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) v += *(const c8_f32x4*)(part + (int64_t)s * rows * pitch + i * 4);
+        wg_store<G>(out + r * F + f, v, f, F);
     }
 }
 
@@ -359,6 +446,12 @@ unsigned int c8_blocks(int64_t lanes) {
     return (unsigned int)(n < 1 ? 1 : (n > 65536 ? 65536 : n));
 }
 
+unsigned int c8_works(int64_t eights) {
+    const int64_t n = (eights + 256 * C8_WORK - 1) / (256 * C8_WORK);
+    TORCH_CHECK(n <= INT_MAX, "checkpoint8: too many values");
+    return (unsigned int)n;
+}
+
 void c8_check(const torch::Tensor& codes, const torch::Tensor& scales, int64_t N, int64_t F) {
     const int64_t Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
     TORCH_CHECK(F > 0 && F <= INT_MAX - C8_GROUP, "checkpoint8: row length out of range");
@@ -367,6 +460,42 @@ void c8_check(const torch::Tensor& codes, const torch::Tensor& scales, int64_t N
                     codes.numel() == N * Fp && scales.numel() == N * (Fp / C8_GROUP),
                 "checkpoint8: codes and scales do not match ", N, " rows of ", F);
     TORCH_CHECK((uintptr_t)codes.data_ptr() % 16 == 0, "checkpoint8: codes must be 16-byte aligned");
+}
+
+// Side of the tiles, and parts that the rows are split into. The least of what was
+// measured, in us: a step of 64 rows takes 2.5 in 256 x 256 tiles (one block a CU),
+// 1.2 in 128 x 128 ones, 1.85 with two of those on a CU; beyond that blocks follow one
+// another; parts are written and read again at 5 TB/s. E.g. 16384 rows, 4096 x 2048:
+// 256 x 2 parts 330 + join, 128 x 1 part 457; 2048 rows, 2048 x 2048: 128 x 1 part 43,
+// 256 x 4 parts 36 + join. 32-bit dy has three products a step, small tiles only
+// (three pieces of dy in LDS) and one block a CU.
+struct WgPlan {
+    int side, splits;
+    int64_t steps;
+};
+
+WgPlan wg_plan(int64_t N, int64_t O, int64_t F, bool pieces) {
+    WgPlan best{128, 1, std::max<int64_t>(1, (N + WG_K - 1) / WG_K)};
+    double least = 1e30;
+    for (int side = pieces ? 128 : 256; side >= 128; side -= 128) {
+        if (side == 256 && (O <= 128 || F <= 128)) continue;
+        const int64_t tiles = ((O + side - 1) / side) * ((F + side - 1) / side);
+        for (int s = 1; s <= 64; ++s) {
+            const int64_t steps = std::max<int64_t>(1, (N + (int64_t)s * WG_K - 1) / ((int64_t)s * WG_K));
+            if (s > 1 && (s - 1) * steps * WG_K >= N) continue;  // an empty part
+            const int64_t blocks = tiles * s;
+            double t = 4;
+            if (side == 256) t += (blocks + 255) / 256 * steps * 2.5;
+            else if (pieces) t += (blocks + 255) / 256 * steps * 3.0;
+            else t += (blocks / 512) * steps * 1.85 + (blocks % 512 == 0 ? 0 : blocks % 512 <= 256 ? steps * 1.2 : steps * 1.85);
+            if (s > 1) t += 2 * s * (double)O * F * 4 / 5e6 + 4;
+            if (t < least) {
+                least = t;
+                best = WgPlan{side, s, steps};
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -381,9 +510,13 @@ void save8_launch(torch::Tensor x, torch::Tensor codes, torch::Tensor scales) {
     auto stream = at::hip::getCurrentHIPStream().stream();
     c8_type(x.scalar_type(), "save8: x", [&](auto e) {
         typedef decltype(e) E;
-        hipLaunchKernelGGL((c8_save<E>), dim3(c8_blocks(N * Fp / 2)), dim3(256), 0, stream, 
-            (const typename E::store*)x.data_ptr(), x.stride(0), (signed char*)codes.data_ptr(),
-            (unsigned char*)scales.data_ptr(), N, (int)F, (int)Fp);
+        const bool vec = F % 8 == 0 && x.stride(0) * x.element_size() % 16 == 0 && (uintptr_t)x.data_ptr() % 16 == 0;
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(c8_works(N * (Fp / 8))), dim3(256), 0, stream, (const typename E::store*)x.data_ptr(),
+                               x.stride(0), (signed char*)codes.data_ptr(), (unsigned char*)scales.data_ptr(), N, (int)F, (int)Fp);
+        };
+        if (vec) go(c8_save<E, true>);
+        else go(c8_save<E, false>);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -398,9 +531,12 @@ void load8_launch(torch::Tensor codes, torch::Tensor scales, torch::Tensor x) {
     auto stream = at::hip::getCurrentHIPStream().stream();
     c8_type(x.scalar_type(), "load8: x", [&](auto e) {
         typedef decltype(e) E;
-        hipLaunchKernelGGL((c8_load<E>), dim3(c8_blocks(N * F)), dim3(256), 0, stream, 
-            (const signed char*)codes.data_ptr(), (const unsigned char*)scales.data_ptr(),
-            (typename E::store*)x.data_ptr(), N, (int)F, (int)Fp);
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(c8_works(N * (Fp / 8))), dim3(256), 0, stream, (const signed char*)codes.data_ptr(),
+                               (const unsigned char*)scales.data_ptr(), (typename E::store*)x.data_ptr(), N, (int)F, (int)Fp);
+        };
+        if (F % 8 == 0 && (uintptr_t)x.data_ptr() % 16 == 0) go(c8_load<E, true>);
+        else go(c8_load<E, false>);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -428,34 +564,28 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     a.O = (int)O;
     a.F = (int)F;
     a.Fp = (int)Fp;
-    // Tiles of 256 x 256 read each operand least; 128 x 128 where those are too few, or
-    // three pieces of dy would not fit LDS.
-    const bool wide = dy.scalar_type() != at::kFloat && O > 128 && F > 128 && ((O + 255) / 256) * ((F + 255) / 256) * ((N + 511) / 512) >= 128;
-    const int64_t side = wide ? 256 : 128;
-    a.tiles_f = (int)((F + side - 1) / side);
-    a.tiles_o = (int)((O + side - 1) / side);
-    const int64_t tiles = (int64_t)a.tiles_f * a.tiles_o;
-    // blocks for the chip (one a CU, or two of the small ones), but at least 256 rows a split
-    int64_t splits = std::min<int64_t>((wide ? 256 : 512) / tiles, (N + 255) / 256);
-    splits = std::max<int64_t>(1, splits);
-    a.per = (((N + splits - 1) / splits) + WG_K - 1) / WG_K * WG_K;
-    a.splits = (int)(a.per > 0 ? std::max<int64_t>(1, (N + a.per - 1) / a.per) : 1);
+    const WgPlan plan = wg_plan(N, O, F, dy.scalar_type() == at::kFloat);
+    const bool wide = plan.side == 256;
+    a.tiles_f = (int)((F + plan.side - 1) / plan.side);
+    a.tiles_o = (int)((O + plan.side - 1) / plan.side);
+    const int64_t tiles = (int64_t)a.tiles_f * a.tiles_o, Fq = (F + 3) / 4 * 4, Oq = (O + 3) / 4 * 4;
+    a.per = plan.steps * WG_K;
+    a.splits = plan.splits;
     TORCH_CHECK(tiles * a.splits <= INT_MAX, "weight_grad8: sizes out of range");
     // whole 16-byte words, and a tile's rows within 31-bit offsets
     const bool aligned = O % 8 == 0 && a.sdy % 8 == 0 && a.sdy >= O && a.sdy <= (1 << 22) && (uintptr_t)a.dy % 16 == 0;
     torch::Tensor part, part_b;
-    const bool join = a.splits > 1;
+    const bool join = a.splits > 1, join_b = db.has_value() && a.splits * a.tiles_f > 1;
+    const auto f32 = dw.options().dtype(at::kFloat);
+    a.dw = dw.data_ptr();
+    a.db = db.has_value() ? db->data_ptr() : nullptr;
     if (join) {
-        auto opt = dw.options().dtype(at::kFloat);
-        part = torch::empty({a.splits, O, F}, opt);
+        part = torch::empty({a.splits, O, Fq}, f32);
         a.dw = part.data_ptr();
-        if (db.has_value()) {
-            part_b = torch::empty({a.splits, O}, opt);
-            a.db = part_b.data_ptr();
-        }
-    } else {
-        a.dw = dw.data_ptr();
-        a.db = db.has_value() ? db->data_ptr() : nullptr;
+    }
+    if (join_b) {
+        part_b = torch::empty({a.splits * a.tiles_f, Oq}, f32);
+        a.db = part_b.data_ptr();
     }
     const dim3 grid((unsigned)(tiles * a.splits));
     c8_type(dy.scalar_type(), "weight_grad8: dy", [&](auto e) {
@@ -468,11 +598,10 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
             }
             if (!wide && aligned) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, true>), grid, dim3(WG_THREADS), 0, stream, a);
             else if (!wide) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, false>), grid, dim3(WG_THREADS), 0, stream, a);
-            if (join) {
-                hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(O * F)), dim3(256), 0, stream, (const float*)part.data_ptr(), (typename G::store*)dw.data_ptr(), O * F, a.splits);
-                if (db.has_value())
-                    hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(O)), dim3(256), 0, stream, (const float*)part_b.data_ptr(), (typename G::store*)db->data_ptr(), O, a.splits);
-            }
+            if (join)
+                hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(O * Fq / 4)), dim3(256), 0, stream, (const float*)part.data_ptr(), (typename G::store*)dw.data_ptr(), O, (int)F, (int)Fq, a.splits);
+            if (join_b)
+                hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(Oq / 4)), dim3(256), 0, stream, (const float*)part_b.data_ptr(), (typename G::store*)db->data_ptr(), (int64_t)1, (int)O, (int)Oq, a.splits * a.tiles_f);
         });
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();

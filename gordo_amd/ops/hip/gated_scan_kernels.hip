@@ -72,15 +72,6 @@ __device__ __forceinline__ void gs_fence(int i) {
     if (W > 1 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
 }
 
-// f(integral_constant 0 .. N-1): for where an instruction wants a constant
-template <int N, int I = 0, class F>
-__device__ __forceinline__ void gs_for(F&& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        gs_for<N, I + 1>(f);
-    }
-}
-
 struct GsArgs {
     const void* p;          // [B][T][P*D], rows at sb, st
     int64_t sb, st;
@@ -333,7 +324,7 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
     const unsigned int scale = c8_scale(top);
     const float mine_inv = c8_inv(scale);
     signed char* to = a.codes + row * a.Dp + dd;
-    gs_for<GS_R>([&](auto n) {
+    c8_for<GS_R>([&](auto n) {
         constexpr int i = decltype(n)::value;
         // row_newbcast: lane i's value to its 16 lanes
         const float inv = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(mine_inv), 0x150 + i, 0xF, 0xF, true));
@@ -496,7 +487,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
 #pragma unroll
             for (int i = 0; i < GS_R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
-            gs_for<GS_R>([&](auto n) {
+            c8_for<GS_R>([&](auto n) {
                 constexpr int i = decltype(n)::value;
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
