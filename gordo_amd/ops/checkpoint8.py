@@ -27,7 +27,6 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ext
 
@@ -85,10 +84,7 @@ def save8(x: torch.Tensor) -> Saved8:
     """The 8-bit codes of ``x``, groups of 32 along its last axis."""
     rows = _rows(x, "x")
     if rows.is_cuda:
-        N, groups = rows.shape[0], -(-rows.shape[1] // GROUP)
-        codes = torch.empty((N, groups * GROUP), dtype=torch.int8, device=rows.device)
-        scales = torch.empty((N, groups), dtype=torch.uint8, device=rows.device)
-        ext().save8(rows, codes, scales)
+        codes, scales = ext().save8(rows)
     else:
         codes, scales = codes_eager(rows.detach())
     return Saved8(codes, scales, x.shape, x.dtype)
@@ -116,8 +112,7 @@ def load8(saved: Saved8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     if saved.codes.is_cuda:
-        out = torch.empty((saved.codes.shape[0], F), dtype=dtype, device=saved.codes.device)
-        ext().load8(saved.codes, saved.scales, out)
+        out = ext().load8(saved.codes, saved.scales, F, dtype)
     else:
         out = values_eager(saved.codes, saved.scales, F).to(dtype)
     return out.reshape(saved.shape)
@@ -152,6 +147,8 @@ def weight_grad8(
 
 
 class _Linear8(torch.autograd.Function):
+    """The CPU form; the GPU's is in hip/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, x, weight, bias):
         y = torch.nn.functional.linear(x, weight.to(x.dtype), None if bias is None else bias.to(x.dtype))
@@ -162,8 +159,8 @@ class _Linear8(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        first_order("linear8")
         weight, codes, scales = ctx.saved_tensors
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
@@ -172,10 +169,15 @@ class _Linear8(torch.autograd.Function):
             saved = Saved8(codes, scales, ctx.x_shape, ctx.x_dtype)
             dw, db = weight_grad8(dy, saved, bias=ctx.needs_input_grad[2], dtype=weight.dtype)
         elif ctx.needs_input_grad[2]:
-            db = dy.flatten(0, -2).sum(0, dtype=torch.float32)
+            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32)
         if db is not None:
             db = db.to(ctx.bias_dtype)
         return dx, dw, db
+
+
+def first_order(what: str) -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: the gradient has no gradient of its own (create_graph)")
 
 
 def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -204,6 +206,7 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
             raise ValueError(f"{what} is on {t.device}, x on {x.device}")
     if torch.is_autocast_enabled(kind):
         x = x.to(torch.get_autocast_dtype(kind))
-        with torch.autocast(kind, enabled=False):
-            return _Linear8.apply(x, weight, bias)
-    return _Linear8.apply(x, weight, bias)
+    if x.is_cuda:
+        return ext().linear8(x, weight, bias)
+    with torch.autocast(kind, enabled=False):
+        return _Linear8.apply(x, weight, bias)

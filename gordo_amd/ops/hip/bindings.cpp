@@ -45,11 +45,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("lstm_fwd_wide256", &lstm_fwd_wide256_launch, "W=256 persistent LSTM forward (column-half split)");
     m.def("lstm_bwd_wide256", &lstm_bwd_wide256_launch, "W=256 reverse-time BPTT cell (+fused dx)");
     m.def("lstm_dw_wide256", &lstm_dw_wide256_launch, "W=256 split-K dWcat 4x4 quadrants + dbias");
-    m.def("gated_scan_fwd", &gated_scan_fwd_launch, "gated linear recurrence over sequences");
-    m.def("gated_scan_bwd", &gated_scan_bwd_launch, "gradient of the gated linear recurrence");
+    m.def("gated_scan", &gated_scan, "gated linear recurrence over sequences, with its gradient");
     m.def("gated_step", &gated_step_launch, "one token of the gated linear recurrence, states in slots");
     m.def("save8", &save8_launch, "8-bit codes with a power-of-two scale for each 32 values");
     m.def("load8", &load8_launch, "the values that 8-bit codes stand for");
+    m.def("linear8", &linear8, "linear layer that keeps its input as 8-bit codes");
     m.def("weight_grad8", &weight_grad8_launch, "weight and bias gradient of a linear layer from 8-bit codes");
     m.attr("WMAX") = 64;
     m.attr("MAXL") = 8;

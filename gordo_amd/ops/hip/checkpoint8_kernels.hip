@@ -419,17 +419,28 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     }
 }
 
-// Sums the splits in their order: [splits][rows][pitch] to [rows][F], four values a lane.
+// Sums of parts in their order: [parts][rows][pitch] to [rows][F], four values a lane.
+struct C8Join {
+    const float* from;
+    void* to;
+    int64_t rows;
+    int F, pitch, parts;
+    unsigned int blocks;
+};
+
+// the weight's sums and the bias's in one launch
 template <class G>
-__global__ __launch_bounds__(256) void c8_join(const float* part, typename G::store* out, int64_t rows, int F, int pitch, int splits) {
-    const int64_t fours = pitch / 4, n = rows * fours;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void c8_join(C8Join w, C8Join b) {
+    const bool bias = blockIdx.x >= w.blocks;
+    const C8Join& j = bias ? b : w;
+    const int64_t fours = j.pitch / 4, n = j.rows * fours;
+    for (int64_t i = (int64_t)(blockIdx.x - (bias ? w.blocks : 0)) * 256 + threadIdx.x; i < n; i += (int64_t)j.blocks * 256) {
         const int64_t r = i / fours;
         const int f = (int)(i - r * fours) * 4;
         c8_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) v += *(const c8_f32x4*)(part + (int64_t)s * rows * pitch + i * 4);
-        wg_store<G>(out + r * F + f, v, f, F);
+        for (int s = 0; s < j.parts; ++s) v += *(const c8_f32x4*)(j.from + (int64_t)s * j.rows * j.pitch + i * 4);
+        wg_store<G>((typename G::store*)j.to + r * j.F + f, v, f, j.F);
     }
 }
 
@@ -500,12 +511,13 @@ WgPlan wg_plan(int64_t N, int64_t O, int64_t F, bool pieces) {
 
 }  // namespace
 
-void save8_launch(torch::Tensor x, torch::Tensor codes, torch::Tensor scales) {
+std::tuple<torch::Tensor, torch::Tensor> save8_launch(torch::Tensor x) {
     TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) == 1 || x.stride(1) == 1), "save8: x must be two-dimensional on the GPU, unit stride last");
     const int64_t N = x.size(0), F = x.size(1), Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
-    c8_check(codes, scales, N, F);
-    TORCH_CHECK(codes.device() == x.device(), "save8: x and its codes are on different devices");
-    if (N == 0) return;
+    TORCH_CHECK(F > 0 && F <= INT_MAX - C8_GROUP, "save8: row length out of range");
+    torch::Tensor codes = at::empty({N, Fp}, x.options().dtype(at::kChar));
+    torch::Tensor scales = at::empty({N, Fp / C8_GROUP}, x.options().dtype(at::kByte));
+    if (N == 0) return {codes, scales};
     const c10::DeviceGuard guard(x.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
     c8_type(x.scalar_type(), "save8: x", [&](auto e) {
@@ -519,14 +531,15 @@ void save8_launch(torch::Tensor x, torch::Tensor codes, torch::Tensor scales) {
         else go(c8_save<E, false>);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
+    return {codes, scales};
 }
 
-void load8_launch(torch::Tensor codes, torch::Tensor scales, torch::Tensor x) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "load8: x must be two-dimensional and contiguous on the GPU");
-    const int64_t N = x.size(0), F = x.size(1), Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
+torch::Tensor load8_launch(torch::Tensor codes, torch::Tensor scales, int64_t F, at::ScalarType dtype) {
+    TORCH_CHECK(codes.dim() == 2 && F > 0, "load8: codes must be two-dimensional");
+    const int64_t N = codes.size(0), Fp = (F + C8_GROUP - 1) / C8_GROUP * C8_GROUP;
     c8_check(codes, scales, N, F);
-    TORCH_CHECK(codes.device() == x.device(), "load8: x and its codes are on different devices");
-    if (N == 0) return;
+    torch::Tensor x = at::empty({N, F}, codes.options().dtype(dtype));
+    if (N == 0) return x;
     const c10::DeviceGuard guard(x.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
     c8_type(x.scalar_type(), "load8: x", [&](auto e) {
@@ -539,6 +552,7 @@ void load8_launch(torch::Tensor codes, torch::Tensor scales, torch::Tensor x) {
         else go(c8_load<E, false>);
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();
+    return x;
 }
 
 void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor scales, torch::Tensor dw,
@@ -598,10 +612,12 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
             }
             if (!wide && aligned) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, true>), grid, dim3(WG_THREADS), 0, stream, a);
             else if (!wide) hipLaunchKernelGGL((c8_weight_grad<E, G, 128, 128, false>), grid, dim3(WG_THREADS), 0, stream, a);
-            if (join)
-                hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(O * Fq / 4)), dim3(256), 0, stream, (const float*)part.data_ptr(), (typename G::store*)dw.data_ptr(), O, (int)F, (int)Fq, a.splits);
-            if (join_b)
-                hipLaunchKernelGGL((c8_join<G>), dim3(c8_blocks(Oq / 4)), dim3(256), 0, stream, (const float*)part_b.data_ptr(), (typename G::store*)db->data_ptr(), (int64_t)1, (int)O, (int)Oq, a.splits * a.tiles_f);
+            if (join || join_b) {
+                C8Join w{}, b{};
+                if (join) w = {(const float*)part.data_ptr(), dw.data_ptr(), O, (int)F, (int)Fq, a.splits, c8_blocks(O * Fq / 4)};
+                if (join_b) b = {(const float*)part_b.data_ptr(), db->data_ptr(), 1, (int)O, (int)Oq, a.splits * a.tiles_f, c8_blocks(Oq / 4)};
+                hipLaunchKernelGGL((c8_join<G>), dim3(w.blocks + b.blocks), dim3(256), 0, stream, w, b);
+            }
         });
     });
     C10_HIP_KERNEL_LAUNCH_CHECK();

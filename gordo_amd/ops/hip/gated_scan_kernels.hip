@@ -910,20 +910,20 @@ void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
     C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-void gated_step_launch(torch::Tensor p, int64_t dim, torch::Tensor state, c10::optional<torch::Tensor> slots,
-                       torch::Tensor out, torch::Tensor y) {
+torch::Tensor gated_step_launch(torch::Tensor p, torch::Tensor state, c10::optional<torch::Tensor> slots,
+                                torch::Tensor out) {
+    TORCH_CHECK(state.dim() == 2, "gated_step: state must be [slots, dim]");
+    const int64_t dim = state.size(1);
     TORCH_CHECK(p.is_cuda() && p.dim() == 2 && p.stride(1) == 1 && dim > 0 &&
                     (p.size(1) == 2 * dim || p.size(1) == 3 * dim) && p.size(0) > 0 && p.size(0) <= INT_MAX && p.size(1) <= INT_MAX,
                 "gated_step: p must be [B, 2 or 3 times dim] on the GPU, unit stride last");
     GsStepArgs a{};
     a.B = (int)p.size(0);
     a.D = (int)dim;
-    TORCH_CHECK(state.dim() == 2 && state.size(1) == dim, "gated_step: state must be [slots, dim]");
     a.S = state.size(0);
     gs_f32(state, a.S * dim, p, "state");
     gs_f32(out, a.S * dim, p, "out");
-    TORCH_CHECK(y.device() == p.device() && y.scalar_type() == p.scalar_type() && y.is_contiguous() &&
-                    y.numel() == (int64_t)a.B * dim, "gated_step: y does not match p");
+    torch::Tensor y = at::empty({a.B, dim}, p.options());
     if (slots.has_value()) {
         TORCH_CHECK(slots->device() == p.device() && slots->is_contiguous() && slots->numel() == a.B &&
                         (slots->scalar_type() == at::kInt || slots->scalar_type() == at::kLong),
@@ -945,4 +945,5 @@ void gated_step_launch(torch::Tensor p, int64_t dim, torch::Tensor state, c10::o
     GsStepCall call{a, threads, at::hip::getCurrentHIPStream().stream()};
     gs_types(p.scalar_type(), pair, p.size(1) / dim, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();
+    return y;
 }

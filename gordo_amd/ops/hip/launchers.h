@@ -140,12 +140,18 @@ void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
                            c10::optional<torch::Tensor> dh_last, torch::Tensor dp,
                            c10::optional<torch::Tensor> dh0);
 
-void gated_step_launch(torch::Tensor p, int64_t dim, torch::Tensor state, c10::optional<torch::Tensor> slots,
-                       torch::Tensor out, torch::Tensor y);
+torch::Tensor gated_step_launch(torch::Tensor p, torch::Tensor state, c10::optional<torch::Tensor> slots,
+                                torch::Tensor out);
 
-void save8_launch(torch::Tensor x, torch::Tensor codes, torch::Tensor scales);
+// (codes, scales)
+std::tuple<torch::Tensor, torch::Tensor> save8_launch(torch::Tensor x);
 
-void load8_launch(torch::Tensor codes, torch::Tensor scales, torch::Tensor x);
+torch::Tensor load8_launch(torch::Tensor codes, torch::Tensor scales, int64_t F, at::ScalarType dtype);
 
 void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor scales, torch::Tensor dw,
                          c10::optional<torch::Tensor> db);
+
+std::tuple<torch::Tensor, torch::Tensor> gated_scan(torch::Tensor p, int64_t dim, c10::optional<torch::Tensor> h0,
+                                                    c10::optional<torch::Tensor> lengths, bool keep8);
+
+torch::Tensor linear8(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> bias);

@@ -23,10 +23,9 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ext
-from .checkpoint8 import GROUP, _DTYPES, codes_eager, values_eager
+from .checkpoint8 import _DTYPES, codes_eager, first_order, values_eager
 
 KEEP_EVERY = 16  # tokens between two kept states
 
@@ -90,57 +89,26 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
     return dp, c
 
 
-# ----------------------------------------------------------------------- kernels
-def _forward(p, dim, h0, lengths, train: bool, keep8: bool):
-    """(y, h_last, states, codes, scales); the last three as far as asked for."""
-    B, T, width = p.shape
-    parts = width // dim
-    if not p.is_cuda:
-        first = torch.zeros(B, dim) if h0 is None else h0
-        y, last, states = _forward_eager(p, dim, first, lengths)
-        codes = scales = None
-        if keep8:
-            codes, scales = codes_eager(p.reshape(B * T * parts, dim))
-        return y, last, states if train else None, codes, scales
-    y = torch.empty((B, T, dim), dtype=p.dtype, device=p.device)
-    last = torch.empty((B, dim), dtype=torch.float32, device=p.device)
-    states = codes = scales = None
-    if train:
-        states = torch.empty((B, -(-T // KEEP_EVERY), dim), dtype=torch.float32, device=p.device)
-    if keep8:
-        groups = -(-dim // GROUP)
-        codes = torch.empty((B * T * parts, groups * GROUP), dtype=torch.int8, device=p.device)
-        scales = torch.empty((B * T * parts, groups), dtype=torch.uint8, device=p.device)
-    ext().gated_scan_fwd(p, dim, h0, lengths, y, last, states, codes, scales)
-    return y, last, states, codes, scales
-
-
 class _GatedScan(torch.autograd.Function):
+    """The CPU form; the GPU's is in hip/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, p, h0, lengths, dim, keep8):
-        y, last, states, codes, scales = _forward(p, dim, h0, lengths, True, keep8)
+        y, last, states = _forward_eager(p, dim, h0, lengths)
+        codes = scales = None
+        if keep8:
+            codes, scales = codes_eager(p.reshape(-1, dim))
         ctx.dim, ctx.p_shape, ctx.p_dtype = dim, p.shape, p.dtype
         ctx.save_for_backward(None if keep8 else p, lengths, states, codes, scales)
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
+        first_order("gated_scan")
         p, lengths, states, codes, scales = ctx.saved_tensors
-        dim, keep8 = ctx.dim, codes is not None
-        dh = dh.contiguous()
-        if not states.is_cuda:
-            kept = values_eager(codes, scales, dim).reshape(ctx.p_shape) if keep8 else p.float()
-            dp, dh0 = _backward_eager(kept, dim, lengths, states, dy, dh)
-            dp = dp.to(ctx.p_dtype)
-        else:
-            if dy.stride(-1) != 1:
-                dy = dy.contiguous()
-            dp = torch.empty(ctx.p_shape, dtype=ctx.p_dtype, device=states.device)
-            dh0 = torch.empty_like(dh) if ctx.needs_input_grad[1] else None
-            # with codes the projection itself is gone; dp stands in for its shape
-            ext().gated_scan_bwd(dp if keep8 else p, dim, lengths, states, codes, scales, dy, dh, dp, dh0)
-        return dp, dh0 if ctx.needs_input_grad[1] else None, None, None, None
+        kept = p.float() if codes is None else values_eager(codes, scales, ctx.dim).reshape(ctx.p_shape)
+        dp, dh0 = _backward_eager(kept, ctx.dim, lengths, states, dy, dh)
+        return dp.to(ctx.p_dtype), dh0, None, None, None
 
 
 # -------------------------------------------------------------------- entry points
@@ -203,9 +171,9 @@ def gated_scan(
         return p[..., :dim] * 1, last
     if p.stride(2) != 1:
         p = p.contiguous()
-    if torch.is_grad_enabled() and (p.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(p, h0, lengths, dim, keep == "int8")
-    return _forward(p, dim, h0, lengths, False, False)[:2]
+    if p.is_cuda:
+        return ext().gated_scan(p, dim, h0, lengths, keep == "int8")
+    return _GatedScan.apply(p, torch.zeros(B, dim) if h0 is None else h0, lengths, dim, keep == "int8")
 
 
 def gated_step(
@@ -251,14 +219,9 @@ def gated_step(
         a, b, n = out.data_ptr(), state.data_ptr(), 4 * S * dim
         if a != b and a < b + n and b < a + n:
             raise ValueError("out overlaps state: pass state itself, or a buffer of its own")
+    if B and p.is_cuda:
+        return ext().gated_step(p if p.stride(1) == 1 else p.contiguous(), state, slots, out)
     y = torch.empty((B, dim), dtype=p.dtype, device=p.device)
-    if B == 0:
-        return y
-    if p.is_cuda:
-        if p.stride(1) != 1:
-            p = p.contiguous()
-        ext().gated_step(p, dim, state, slots, out, y)
-        return y
     pf = p.detach().float()
     new = {}
     for b in range(B):

@@ -17,6 +17,7 @@ try:
     os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
     hip_sources = [
         "gordo_amd/ops/hip/bindings.cpp",
+        "gordo_amd/ops/hip/autograd.cpp",
         "gordo_amd/ops/hip/hourglass_kernels.hip",
         "gordo_amd/ops/hip/lstm_kernels.hip",
         "gordo_amd/ops/hip/lstm_h32_kernels.hip",

@@ -283,17 +283,21 @@ def test_linear8_parts(device):
     y = linear8(x, w.clone().requires_grad_())
     assert torch.allclose(y, x @ w.t(), atol=1e-4)
     xr = x.clone().requires_grad_()
-    y = linear8(xr, w, b)
-    assert y.grad_fn.saved_tensors[1] is None  # nothing of x is kept where no weight asks
+    kept = []
+    watch = torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t)
+    with watch:
+        y = linear8(xr, w, b)
+    assert [t.shape for t in kept] == [w.shape]  # nothing of x where no weight asks
     dx = torch.autograd.grad(y.sum(), xr)[0]
     assert torch.allclose(dx, w.sum(0).expand(30, 64), atol=1e-4)
     br = b.clone().requires_grad_()
     db = torch.autograd.grad(linear8(x, w, br).sum(), br)[0]
     assert torch.allclose(db, torch.full((8,), 30.0, device=device))
     wr = w.clone().requires_grad_()
-    y = linear8(x, wr, b)
-    kept = y.grad_fn.saved_tensors
-    assert {t.dtype for t in kept[1:]} == {torch.int8, torch.uint8}
+    kept.clear()
+    with watch:
+        y = linear8(x, wr, b)
+    assert {t.dtype for t in kept if t.shape != w.shape} == {torch.int8, torch.uint8} and len(kept) == 3
     with torch.no_grad():
         assert linear8(x, wr, b).grad_fn is None
 
@@ -310,6 +314,13 @@ def test_linear8_under_autocast(device):
     assert dx.dtype == torch.float32 and dw.dtype == torch.float32
     want = kept8(x.to(torch.bfloat16)).sum(0).expand(12, 40)
     close(dw, want, kept8(x.to(torch.bfloat16)).abs().sum(0).expand(12, 40), 20, "dw")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_linear8_no_gradient_of_the_gradient(device):
+    x = torch.randn(4, 6, device=device, requires_grad=True)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(linear8(x, torch.randn(3, 6, device=device)).sum(), x, create_graph=True)
 
 
 # ------------------------------------------------------------- the block, together

@@ -270,6 +270,13 @@ def test_scan_refuses():
             bad()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_gradient_of_the_gradient(device):
+    p = torch.randn(1, 4, 6, device=device, requires_grad=True)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(gated_scan(p, 3)[0].sum(), p, create_graph=True)
+
+
 # ----------------------------------------------------------------------- the step
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
