@@ -93,6 +93,8 @@ struct GsArgs {
     int tps;                // lanes of one sequence
     int nJ;                 // blocks' tiles along T
     int groups;             // 64-lane groups of channels
+    int seqs;               // staged: sequences of a wave
+    int pitch_p, pitch_y;   // staged: bytes of a sequence's tile of p and of y in LDS
     // chained blocks (null: a block walks all its tiles)
     unsigned int* ticket;
     unsigned long long* agg;  // [nJ][groups][V][64]: a tile's (A, H), all ones until it is there
@@ -109,7 +111,56 @@ __device__ __forceinline__ int gs_len(const GsArgs& a, int b) {
 struct GsLane {
     int b, d, len;
     bool live;  // has a channel
+    int seq;    // staged: which of the wave's sequences
 };
+
+// staged: a wave has whole sequences
+__device__ __forceinline__ GsLane gs_lane_staged(const GsArgs& a, int64_t cg, int lane) {
+    GsLane l;
+    l.seq = lane / a.tps;
+    l.d = lane - l.seq * a.tps;
+    const int64_t b = cg * a.seqs + l.seq;
+    l.live = l.seq < a.seqs && b < a.B && l.d < a.D;
+    l.seq = min(l.seq, a.seqs - 1);
+    l.b = (int)min(b, (int64_t)a.B - 1);
+    l.d = min(l.d, a.D - 1);
+    l.len = l.live ? gs_len(a, l.b) : a.T;
+    return l;
+}
+
+// ---------------------------------------------------------------------------
+// Staging of narrow rows. Rows of 25 or 50 channels start and end inside a memory
+// sector; written row by row, every sector is written in pieces (2.8 TB/s at 25
+// channels against 5.3 at 32). But a sequence's tile of GS_R rows is one run of bytes:
+// it goes through LDS, and memory sees whole words of the run, 256 bytes at a time.
+// A run starts at any 2-byte address; in LDS it keeps its place within a word, so a
+// word of memory is a word of LDS. A load may take the other half of the run's first
+// or last word along (memory of the same aligned 4 bytes); a store leaves it alone.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void gs_stage_in(const char* run, int bytes, char* lds, int lane) {
+    const int n = ((int)((uintptr_t)run & 3) + bytes + 3) >> 2;
+    const unsigned int* from = (const unsigned int*)(run - ((uintptr_t)run & 3));
+    for (int w = 0; w < n; w += 64)
+        if (w + lane < n)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + w + lane),
+                                             (__attribute__((address_space(3))) void*)(lds + 4 * w), 4, 0, 0);
+}
+
+__device__ __forceinline__ void gs_stage_out(char* run, int bytes, const char* lds, int lane) {
+    const int skip = (int)((uintptr_t)run & 3), end = skip + bytes, n = (end + 3) >> 2;
+    char* to = run - skip;
+    for (int w = lane; w < n; w += 64) {
+        const unsigned int v = *(const unsigned int*)(lds + 4 * w);
+        if (4 * w >= skip && 4 * w + 4 <= end) *(unsigned int*)(to + 4 * w) = v;
+        else if (4 * w < skip) *(unsigned short*)(to + 4 * w + 2) = (unsigned short)(v >> 16);
+        else *(unsigned short*)(to + 4 * w) = (unsigned short)v;
+    }
+}
+
+// What was loaded into LDS is there, and what was read from it is in registers, for the
+// one wave of the block. Said outright: a barrier of one wave waits for nothing.
+__device__ __forceinline__ void gs_staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void gs_taken() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <int V>
 __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
@@ -117,6 +168,7 @@ __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
     int64_t b = id / a.tps;
     l.d = (int)(id - b * a.tps) * V;
     l.live = b < a.B && l.d < a.D;
+    l.seq = 0;
     l.b = b < a.B ? (int)b : a.B - 1;   // lanes without a channel read one that exists
     l.d = l.d < a.D ? l.d : a.D - V;
     l.len = l.live ? gs_len(a, l.b) : a.T;
@@ -342,15 +394,17 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
         a.scales[(row + i * step) * (a.Dp / C8_GROUP) + dd / C8_GROUP] = (unsigned char)scale;
 }
 
-template <class E, int V, int P, bool KEEP, int W>
+template <class E, int V, int P, bool KEEP, int W, bool STAGE = false>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(GsArgs a) {
     typedef GsPack<E, V> pack;
+    static_assert(!STAGE || (W == 1 && V == 1), "staged: a wave alone, a channel a lane");
+    extern __shared__ __attribute__((aligned(16))) char gs_lds[];
     __shared__ GsChain<V, W> chain;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
-    const GsLane l = gs_lane<V>(a, id);
+    const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
     typename E::store* y = (typename E::store*)a.y + (int64_t)l.b * a.T * a.D + l.d;
@@ -359,14 +413,44 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = a.h0 != nullptr ? a.h0[(int64_t)l.b * a.D + l.d + v] : 0.f;
 
+    constexpr int ES = sizeof(typename E::store);
+    char* const lds_y = gs_lds + a.seqs * a.pitch_p;
+    // this lane's place in a sequence's tile, p's and y's
+    const char* mine_p = nullptr;
+    char* mine_y = nullptr;
+    if constexpr (STAGE) {
+        // a tile is GS_R rows: its start within a word is the sequence's own, tile after tile
+        mine_p = gs_lds + l.seq * a.pitch_p + (int)((uintptr_t)((const typename E::store*)a.p + l.b * a.sb) & 3) + l.d * ES;
+        mine_y = lds_y + l.seq * a.pitch_y + (int)((uintptr_t)((const typename E::store*)a.y + (int64_t)l.b * a.T * a.D) & 3) + l.d * ES;
+    }
+    auto stage = [&](int tile) {
+        for (int s = 0; s < a.seqs; ++s) {
+            const int64_t b = cg * (int64_t)a.seqs + s, t0 = (int64_t)tile * GS_R;
+            if (b < a.B && t0 < a.T)
+                gs_stage_in((const char*)((const typename E::store*)a.p + b * a.sb + t0 * a.st), min(GS_R, a.T - (int)t0) * P * a.D * ES,
+                            gs_lds + s * a.pitch_p, lane);
+        }
+    };
+    if constexpr (STAGE) stage(0);
+
     for (; j < end; ++j) {
         const int tile = j * W + wid, t0 = tile * GS_R;
         pack raw[P][GS_R];
+        if constexpr (STAGE) {
+            gs_staged();
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
-            const int t = min(t0 + i, a.T - 1);
+            for (int i = 0; i < GS_R; ++i)
 #pragma unroll
-            for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
+                for (int q = 0; q < P; ++q) raw[q][i].load((const typename E::store*)(mine_p + (i * P + q) * a.D * ES));
+            gs_taken();
+            stage(tile + 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) {
+                const int t = min(t0 + i, a.T - 1);
+#pragma unroll
+                for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
+            }
         }
         if (!__all(l.len >= t0 + GS_R)) {
 #pragma unroll
@@ -395,12 +479,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
         }
         if constexpr (KEEP) {
             const int64_t row = ((int64_t)l.b * a.T + t0) * P;
-            const int dd = (int)(id % a.tps) * V;  // channel, padding included
+            // channel, padding included, and whether it is one
+            const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
+            const bool kept = STAGE ? lane / a.tps < a.seqs && cg * (int64_t)a.seqs + lane / a.tps < a.B : id < (int64_t)a.B * a.tps;
 #pragma unroll
             for (int q = 0; q < P; ++q) {
 #pragma unroll
                 for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
-                gs_encode<E, V>(a, raw[q], l.live, id < (int64_t)a.B * a.tps, row + q, P, a.T - t0, dd, lane);
+                gs_encode<E, V>(a, raw[q], l.live, kept, row + q, P, a.T - t0, dd, lane);
             }
         }
 #pragma unroll
@@ -416,10 +502,22 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                     out[v] *= z * gs_sigmoid(z);
                 }
             }
-            if (l.live && t0 + i < l.len) pack::put(y + (int64_t)(t0 + i) * a.D, out);
+            if constexpr (STAGE) {
+                if (t0 + i >= l.len) out[0] = 0.f;
+                if (l.live) pack::put((typename E::store*)(mine_y + i * a.D * ES), out);
+            } else if (l.live && t0 + i < l.len) {
+                pack::put(y + (int64_t)(t0 + i) * a.D, out);
+            }
             gs_fence<W>(i);
         }
-        if (l.live) {
+        if constexpr (STAGE) {
+            gs_taken();
+            for (int s = 0; s < a.seqs; ++s) {
+                const int64_t b = cg * (int64_t)a.seqs + s;
+                if (b < a.B)
+                    gs_stage_out((char*)((typename E::store*)a.y + (b * a.T + t0) * a.D), min(GS_R, a.T - t0) * a.D * ES, lds_y + s * a.pitch_y, lane);
+            }
+        } else if (l.live) {
             const float zero[V] = {};
             for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
         }
@@ -443,16 +541,17 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 // The chain carries c, from the last tile to the first. Kept codes are decoded as
 // they are loaded, to bf16, in which they are exact.
 // ---------------------------------------------------------------------------
-template <class E, int V, int P, bool KEEP, int W>
+template <class E, int V, int P, bool KEEP, int W, bool STAGE = false>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(GsArgs a) {
     typedef GsPack<E, V> pack;
+    extern __shared__ __attribute__((aligned(16))) char gs_lds[];
     typedef typename std::conditional<KEEP, C8Bf16, E>::type K;  // type of the kept projection in registers
     __shared__ GsChain<V, W> chain;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
-    const GsLane l = gs_lane<V>(a, id);
+    const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;
     const int64_t row0 = (int64_t)l.b * a.T;
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
@@ -463,16 +562,54 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = a.dh_last != nullptr ? a.dh_last[(int64_t)l.b * a.D + l.d + v] : 0.f;
 
+    // LDS, staged: a tile of p (not of codes: their rows are whole sectors), one of dy, and
+    // one of dp to go out
+    constexpr int ES = sizeof(typename E::store);
+    char* const lds_dy = gs_lds + (KEEP ? 0 : a.seqs * a.pitch_p);
+    char* const lds_dp = lds_dy + a.seqs * a.pitch_y;
+    const char *mine_p = nullptr, *mine_dy = nullptr;
+    char* mine_dp = nullptr;
+    if constexpr (STAGE) {
+        mine_p = gs_lds + l.seq * a.pitch_p + (int)((uintptr_t)((const typename E::store*)a.p + l.b * a.sb) & 3) + l.d * ES;
+        mine_dy = lds_dy + l.seq * a.pitch_y + (int)((uintptr_t)((const typename E::store*)a.dy + l.b * a.dsb) & 3) + l.d * ES;
+        mine_dp = lds_dp + l.seq * a.pitch_p + (int)((uintptr_t)((const typename E::store*)a.dp + row0 * P * a.D) & 3) + l.d * ES;
+    }
+    auto stage = [&](int tile) {
+        if (tile < 0) return;
+        const int t0 = tile * GS_R, rows = min(GS_R, a.T - t0);
+        for (int s = 0; s < a.seqs; ++s) {
+            const int64_t b = cg * (int64_t)a.seqs + s;
+            if (b >= a.B) break;
+            if constexpr (!KEEP)
+                gs_stage_in((const char*)((const typename E::store*)a.p + b * a.sb + t0 * a.st), rows * P * a.D * ES, gs_lds + s * a.pitch_p, lane);
+            gs_stage_in((const char*)((const typename E::store*)a.dy + b * a.dsb + t0 * a.dst), rows * a.D * ES, lds_dy + s * a.pitch_y, lane);
+        }
+    };
+    if constexpr (STAGE) stage(a.nJ - 1);
+
     for (; j < end; ++j) {
         const int tile = (a.nJ - 1 - j) * W + wid, t0 = tile * GS_R;
         GsPack<K, V> raw[P][GS_R];
         pack up[GS_R];
+        if constexpr (STAGE) {
+            gs_staged();
+#pragma unroll
+            for (int i = 0; i < GS_R; ++i) {
+                up[i].load((const typename E::store*)(mine_dy + i * a.D * ES));
+                if constexpr (!KEEP)
+#pragma unroll
+                    for (int q = 0; q < P; ++q) raw[q][i].load((const typename E::store*)(mine_p + (i * P + q) * a.D * ES));
+            }
+            gs_taken();
+            stage(tile - 1);
+        }
         if constexpr (KEEP) {
             // lane i of 16 has the scale of token i
             float step[P];
             const int ti = min(t0 + (lane & 15), a.T - 1);
             const int ng = a.Dp / C8_GROUP;
-            const int dd = (int)(id % a.tps) * V;  // the group's lanes stay together, padding included
+            // the group's lanes stay together, padding included
+            const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
 #pragma unroll
             for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[((row0 + ti) * P + q) * ng + dd / C8_GROUP]);
 #pragma unroll
@@ -485,8 +622,9 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                     else raw[q][i].w = *(const unsigned char*)from;
                 }
             }
+            if constexpr (!STAGE)
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
+                for (int i = 0; i < GS_R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
             c8_for<GS_R>([&](auto n) {
                 constexpr int i = decltype(n)::value;
 #pragma unroll
@@ -500,7 +638,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                     else raw[q][i].w = __float_as_uint(f0) >> 16;
                 }
             });
-        } else {
+        } else if constexpr (!STAGE) {
 #pragma unroll
             for (int i = 0; i < GS_R; ++i) {
                 const int t = min(t0 + i, a.T - 1);
@@ -590,7 +728,13 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                     out[0][v] = gk;
                     out[1][v] = (hp - x) * fmaf(-kk, gk, gk);
                 }
-                if (l.live && t0 + i < l.len) {
+                if constexpr (STAGE) {
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        if (t0 + i >= l.len) out[q][0] = 0.f;
+                        if (l.live) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), out[q]);
+                    }
+                } else if (l.live && t0 + i < l.len) {
 #pragma unroll
                     for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)(t0 + i) * P + q) * a.D, out[q]);
                 }
@@ -599,7 +743,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = first[v];
         }
-        if (l.live) {
+        if constexpr (STAGE) {
+            gs_taken();
+            for (int s = 0; s < a.seqs; ++s) {
+                const int64_t b = cg * (int64_t)a.seqs + s;
+                if (b < a.B)
+                    gs_stage_out((char*)((typename E::store*)a.dp + (b * a.T + t0) * P * a.D), min(GS_R, a.T - t0) * P * a.D * ES, lds_dp + s * a.pitch_p, lane);
+            }
+        } else if (l.live) {
             const float zero[V] = {};
             for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t)
 #pragma unroll
@@ -726,17 +877,35 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
 // and more than a few tiles, blocks are chained along time. Forward without codes
 // fits 128 registers a lane: blocks of 8 waves, 4 waves a SIMD. The codes and the
 // backward pass need up to 168: blocks of 4, 3 waves a SIMD.
+// Where a wave walks alone, narrow rows that are not whole sectors (64 bytes) go
+// through LDS: 8192 sequences of 144 tokens, 25 channels in bf16, take 53 + 75 us that way,
+// forward and backward, and 64 + 102 row by row.
 struct GsPlan {
     int W;
     unsigned int blocks;
     torch::Tensor space;
+    bool staged;
+    size_t lds;
 };
 
-GsPlan gs_plan(GsArgs& a, int V, int many, const torch::Tensor& p, hipStream_t stream) {
-    GsPlan plan;
+GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hipStream_t stream) {
+    GsPlan plan{};
     const int64_t groups = ((int64_t)a.B * a.tps + 63) / 64;
     TORCH_CHECK(groups <= INT_MAX && a.T <= (1 << 30), "gated_scan: sizes of p out of range");
     plan.W = a.T <= GS_R || groups >= 2048 ? 1 : many;
+    const int es = (int)p.element_size(), lanes = a.codes != nullptr ? a.Dp : a.D;
+    if (plan.W == 1 && a.D <= 64 && a.D * es % 64 != 0 && (a.T == 1 || (a.st == (int64_t)parts * a.D && (a.dy == nullptr || a.dst == a.D)))) {
+        plan.staged = true;
+        a.tps = lanes;
+        a.seqs = 64 / lanes;
+        a.pitch_p = (GS_R * parts * a.D * es + 7) / 4 * 4;
+        a.pitch_y = (GS_R * a.D * es + 7) / 4 * 4;
+        a.nJ = (a.T + GS_R - 1) / GS_R;
+        plan.blocks = (unsigned int)((a.B + a.seqs - 1) / a.seqs);
+        const int p_in = a.dy != nullptr && a.codes != nullptr ? 0 : a.pitch_p;
+        plan.lds = (size_t)a.seqs * (p_in + a.pitch_y + (a.dy != nullptr ? a.pitch_p : 0));
+        return plan;
+    }
     a.groups = (int)groups;
     a.nJ = (a.T + plan.W * GS_R - 1) / (plan.W * GS_R);
     int64_t blocks = groups;
@@ -762,7 +931,8 @@ struct GsFwdCall {
     hipStream_t stream;
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.W == 1) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        if (plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        else if (plan.W == 1) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, KEEP ? 4 : 8>), dim3(plan.blocks), dim3(KEEP ? 256 : 512), 0, stream, a);
     }
     template <class E, int V, int P>
@@ -778,7 +948,8 @@ struct GsBwdCall {
     hipStream_t stream;
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.W == 1) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        if (plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        else if (plan.W == 1) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 4>), dim3(plan.blocks), dim3(256), 0, stream, a);
     }
     template <class E, int V, int P>
@@ -862,7 +1033,7 @@ void gated_scan_fwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
     a.tps = a.codes != nullptr ? a.Dp / V : a.D / V;
     const c10::DeviceGuard guard(p.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
-    const GsPlan plan = gs_plan(a, V, a.codes != nullptr ? 4 : 8, p, stream);
+    const GsPlan plan = gs_plan(a, V, a.codes != nullptr ? 4 : 8, (int)parts, p, stream);
     GsFwdCall call{a, plan, stream};
     gs_types(p.scalar_type(), pair, parts, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -904,7 +1075,7 @@ void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
     a.tps = a.codes != nullptr ? a.Dp / V : a.D / V;
     const c10::DeviceGuard guard(p.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
-    const GsPlan plan = gs_plan(a, V, 4, p, stream);
+    const GsPlan plan = gs_plan(a, V, 4, (int)parts, p, stream);
     GsBwdCall call{a, plan, stream};
     gs_types(p.scalar_type(), pair, parts, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -377,6 +377,9 @@ def test_step_refuses():
         (600, 650, 120),  # many of them
         (2200, 70, 62),   # a wave walks alone
         (70000, 3, 4),    # a tile is more than a sequence
+        (9000, 37, 25),   # narrow rows, staged: runs at every 2-byte place
+        (6000, 35, 50),
+        (4500, 33, 33),   # a sequence a wave
     ],
 )
 def test_every_way_of_splitting(B, T, D, dtype, gate, keep):
@@ -384,6 +387,20 @@ def test_every_way_of_splitting(B, T, D, dtype, gate, keep):
     lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(2)).cuda()
     lengths[-1] = T
     check(p, D, h0, lengths, dy, dh, keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [0, 1, 2, 3])
+def test_narrow_rows_in_a_larger_buffer(first):
+    """Dense sequences that start anywhere: what lies between them is left alone."""
+    B, T, D = 7000, 20, 25
+    p, h0, dy, dh = inputs(B, T, D, torch.bfloat16, "cuda", gate=False)
+    n = T * 2 * D
+    buf = torch.full((B, n + 3), float("nan"), dtype=p.dtype, device="cuda")
+    view = buf.as_strided((B, T, 2 * D), (n + 3, 2 * D, 1), first)
+    view.copy_(p)
+    a, b = check(view, D, h0, None, dy, dh), check(p, D, h0, None, dy, dh)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2][0], b[2][0])
 
 
 @pytest.mark.gpu
