@@ -37,7 +37,7 @@ Scan scan(const Tensor& p, int64_t dim, const c10::optional<Tensor>& h0, const c
     if (keep8) {
         const int64_t rows = B * T * (p.size(2) / dim), groups = (dim + kGroup - 1) / kGroup;
         s.codes = at::empty({rows, groups * kGroup}, p.options().dtype(at::kChar));
-        s.scales = at::empty({rows, groups}, p.options().dtype(at::kByte));
+        s.scales = at::empty({B, (T + kEvery - 1) / kEvery, p.size(2) / dim, groups, kEvery}, p.options().dtype(at::kByte));
     }
     gated_scan_fwd_launch(p, dim, h0, lengths, s.y, s.last, some(s.states), some(s.codes), some(s.scales));
     return s;

@@ -491,7 +491,7 @@ WgPlan wg_plan(int64_t N, int64_t O, int64_t F, bool pieces) {
     for (int side = pieces ? 128 : 256; side >= 128; side -= 128) {
         if (side == 256 && (O <= 128 || F <= 128)) continue;
         const int64_t tiles = ((O + side - 1) / side) * ((F + side - 1) / side);
-        for (int s = 1; s <= 64; ++s) {
+        for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
             const int64_t steps = std::max<int64_t>(1, (N + (int64_t)s * WG_K - 1) / ((int64_t)s * WG_K));
             if (s > 1 && (s - 1) * steps * WG_K >= N) continue;  // an empty part
             const int64_t blocks = tiles * s;

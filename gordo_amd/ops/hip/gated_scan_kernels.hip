@@ -82,7 +82,7 @@ struct GsArgs {
     const void* lengths;    // [B] or null
     int lengths64;
     signed char* codes;     // [B][T][P][Dp] or null
-    unsigned char* scales;  // [B][T][P][Dp / 32]
+    unsigned char* scales;  // [B][nT][P][Dp / 32][GS_R]: a tile's scales of a group lie together
     // backward
     const void* dy;         // [B][T][D], rows at dsb, dst
     int64_t dsb, dst;
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void gs_clear(uint4* to, int64_t n) {
 // at once and stored once, and come back to the lanes by a broadcast.
 template <class E, int V>
 __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&raw)[GS_R], bool live, bool mine, int64_t row,
-                                          int64_t step, int left, int dd, int lane) {
+                                          int64_t step, int64_t group, int left, int dd, int lane) {
     unsigned int top = 0;
 #pragma unroll
     for (int i = 0; i < GS_R; ++i) {
@@ -389,9 +389,8 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
         to += step * a.Dp;
         if constexpr (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     });
-    const int i = lane & 15;
-    if (mine && i < left && (V == 2 || (lane & 16) == 0))
-        a.scales[(row + i * step) * (a.Dp / C8_GROUP) + dd / C8_GROUP] = (unsigned char)scale;
+    // 64 bytes in a row from a wave: a scale at its token's place would be a 4-byte write
+    if (mine && (V == 2 || (lane & 16) == 0)) a.scales[(group + dd / C8_GROUP) * GS_R + (lane & 15)] = (unsigned char)scale;
 }
 
 template <class E, int V, int P, bool KEEP, int W, bool STAGE = false>
@@ -486,7 +485,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             for (int q = 0; q < P; ++q) {
 #pragma unroll
                 for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
-                gs_encode<E, V>(a, raw[q], l.live, kept, row + q, P, a.T - t0, dd, lane);
+                gs_encode<E, V>(a, raw[q], l.live, kept && tile < nT, row + q, P, (((int64_t)l.b * nT + tile) * P + q) * (a.Dp / C8_GROUP), a.T - t0, dd, lane);
             }
         }
 #pragma unroll
@@ -606,12 +605,11 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         if constexpr (KEEP) {
             // lane i of 16 has the scale of token i
             float step[P];
-            const int ti = min(t0 + (lane & 15), a.T - 1);
-            const int ng = a.Dp / C8_GROUP;
+            const int64_t group = ((int64_t)l.b * nT + min(tile, nT - 1)) * P * (a.Dp / C8_GROUP);
             // the group's lanes stay together, padding included
             const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
 #pragma unroll
-            for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[((row0 + ti) * P + q) * ng + dd / C8_GROUP]);
+            for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[(group + (q * a.Dp + dd) / C8_GROUP) * GS_R + (lane & 15)]);
 #pragma unroll
             for (int i = 0; i < GS_R; ++i) {
                 const int t = min(t0 + i, a.T - 1);
@@ -994,11 +992,11 @@ void gs_lengths(GsArgs& a, const c10::optional<torch::Tensor>& lengths, const to
 void gs_codes(GsArgs& a, const c10::optional<torch::Tensor>& codes, const c10::optional<torch::Tensor>& scales,
               const torch::Tensor& p, int64_t parts) {
     if (!codes.has_value()) return;
-    const int64_t rows = p.size(0) * p.size(1) * parts;
+    const int64_t rows = p.size(0) * p.size(1) * parts, groups = p.size(0) * ((a.T + GS_R - 1) / GS_R) * parts * (a.Dp / C8_GROUP);
     TORCH_CHECK(scales.has_value() && codes->device() == p.device() && scales->device() == p.device() &&
                     codes->scalar_type() == at::kChar && scales->scalar_type() == at::kByte &&
                     codes->is_contiguous() && scales->is_contiguous() &&
-                    codes->numel() == rows * a.Dp && scales->numel() == rows * (a.Dp / C8_GROUP),
+                    codes->numel() == rows * a.Dp && scales->numel() == groups * GS_R,
                 "gated_scan: codes and scales do not match p");
     a.codes = (signed char*)codes->data_ptr();
     a.scales = (unsigned char*)scales->data_ptr();
