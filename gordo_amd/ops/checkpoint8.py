@@ -166,12 +166,9 @@ class _Linear8(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = torch.matmul(dy, weight.to(ctx.x_dtype))
         if ctx.needs_input_grad[1]:
-            saved = Saved8(codes, scales, ctx.x_shape, ctx.x_dtype)
-            dw, db = weight_grad8(dy, saved, bias=ctx.needs_input_grad[2], dtype=weight.dtype)
-        elif ctx.needs_input_grad[2]:
-            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32)
-        if db is not None:
-            db = db.to(ctx.bias_dtype)
+            dw, _ = weight_grad8(dy, Saved8(codes, scales, ctx.x_shape, ctx.x_dtype), dtype=weight.dtype)
+        if ctx.needs_input_grad[2]:
+            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
         return dx, dw, db
 
 

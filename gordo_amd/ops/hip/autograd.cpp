@@ -94,6 +94,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &weight = saved[0], &codes = saved[1], &dy = grads[0];
         const bool bias = ctx->saved_data["bias"].toBool();
+        const auto bias_type = (at::ScalarType)ctx->saved_data["bias_type"].toInt();
         Tensor dx, dw, db;
         if (ctx->saved_data["x"].toBool()) dx = at::matmul(dy, weight.to(dy.scalar_type()));
         const int64_t O = weight.size(0), F = weight.size(1);
@@ -101,12 +102,10 @@ struct Linear8 : torch::autograd::Function<Linear8> {
         if (codes.defined()) {
             if (O > 1 && rows.stride(1) != 1) rows = rows.contiguous();
             dw = at::empty({O, F}, weight.options());
-            if (bias) db = at::empty({O}, weight.options());
+            if (bias && bias_type == weight.scalar_type()) db = at::empty({O}, weight.options());
             weight_grad8_launch(rows, codes, saved[2], dw, some(db));
-        } else if (bias) {
-            db = rows.sum(0, false, at::kFloat);
         }
-        if (bias) db = db.to((at::ScalarType)ctx->saved_data["bias_type"].toInt());
+        if (bias && !db.defined()) db = rows.sum(0, false, at::kFloat).to(bias_type);
         return {dx, dw, db};
     }
 };

@@ -245,10 +245,12 @@ __device__ __forceinline__ void gs_place(const GsArgs& a, GsChain<V, W>& s, int&
 // block's first tile; of the chain's first block where blocks are chained), and,
 // where a block walks on, in `carry` the state after its last tile. `mine`: this wave's map; `order`:
 // this wave's place in the block, 0 first. j counts tiles in the chain's order.
-template <int V, int W>
+// `meanwhile` is done after this block's map is out and before others' are waited for.
+template <int V, int W, class F>
 __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int cg, int j, int order, int lane,
-                                        const float2 (&mine)[V], float (&carry)[V], float (&in)[V]) {
+                                        const float2 (&mine)[V], float (&carry)[V], float (&in)[V], F&& meanwhile) {
     if constexpr (W == 1) {
+        meanwhile();
 #pragma unroll
         for (int v = 0; v < V; ++v) in[v] = carry[v];
         return;
@@ -271,6 +273,17 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
             }
         }
     };
+    const int i = j % GS_LB, g = j / GS_LB;
+    const bool more = j + 1 < a.nJ;
+    if (a.ticket != nullptr && order == W - 1 && i < GS_LB - 1 && more) {
+        parts();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            gs_publish(a.agg + (((int64_t)j * a.groups + cg) * V + v) * 64 + lane, all[v]);
+            all[v] = float2{1.f, 0.f};
+        }
+    }
+    meanwhile();
     if (a.ticket == nullptr) {
         parts();
 #pragma unroll
@@ -279,16 +292,6 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
             carry[v] = fmaf(all[v].x, carry[v], all[v].y);
         }
         return;
-    }
-    const int i = j % GS_LB, g = j / GS_LB;
-    const bool more = j + 1 < a.nJ;
-    if (order == W - 1 && i < GS_LB - 1 && more) {
-        parts();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            gs_publish(a.agg + (((int64_t)j * a.groups + cg) * V + v) * 64 + lane, all[v]);
-            all[v] = float2{1.f, 0.f};
-        }
     }
     // the wave's share of the blocks before, since the last link
     int spins = 0;
@@ -471,22 +474,24 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             }
             gs_fence<W>(i);
         }
-        gs_join<V, W>(a, chain, cg, j, wid, lane, m, carry, h);
+        // the codes are made while the state is on its way
+        gs_join<V, W>(a, chain, cg, j, wid, lane, m, carry, h, [&] {
+            if constexpr (KEEP) {
+                const int64_t row = ((int64_t)l.b * a.T + t0) * P;
+                // channel, padding included, and whether it is one
+                const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
+                const bool kept = STAGE ? lane / a.tps < a.seqs && cg * (int64_t)a.seqs + lane / a.tps < a.B : id < (int64_t)a.B * a.tps;
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+#pragma unroll
+                    for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
+                    gs_encode<E, V>(a, raw[q], l.live, kept && tile < nT, row + q, P, (((int64_t)l.b * nT + tile) * P + q) * (a.Dp / C8_GROUP), a.T - t0, dd, lane);
+                }
+            }
+        });
         if (a.states != nullptr && l.live && tile < nT) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
-        }
-        if constexpr (KEEP) {
-            const int64_t row = ((int64_t)l.b * a.T + t0) * P;
-            // channel, padding included, and whether it is one
-            const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
-            const bool kept = STAGE ? lane / a.tps < a.seqs && cg * (int64_t)a.seqs + lane / a.tps < a.B : id < (int64_t)a.B * a.tps;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-#pragma unroll
-                for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
-                gs_encode<E, V>(a, raw[q], l.live, kept && tile < nT, row + q, P, (((int64_t)l.b * nT + tile) * P + q) * (a.Dp / C8_GROUP), a.T - t0, dd, lane);
-            }
         }
 #pragma unroll
         for (int i = 0; i < GS_R; ++i) {
@@ -677,7 +682,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
             gs_fence<W>(i);
         }
-        gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c);
+        gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c, [] {});
         // the states of half a tile at a time: the first half's are computed twice
         // (two operations each), and half of them in registers is enough
         constexpr int HALF = GS_R / 2;

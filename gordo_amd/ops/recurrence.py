@@ -190,7 +190,8 @@ def gated_step(
     slots  [B] int32 or int64: the slot of each row; None: row b has slot b, and
            S is B. A slot outside 0..S-1 names no state: its row is padding, y is
            0 there and nothing is written. Rows with the same slot are applied
-           one after the other in their order.
+           one after the other in their order. (Every row is looked for in
+           all others: some thousand rows a call, not a hundred thousand.)
     out    where the new states go: ``state`` itself (None), or a buffer of its
            shape that does not overlap it; slots that no row names are left as
            they are there.

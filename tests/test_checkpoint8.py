@@ -303,6 +303,19 @@ def test_linear8_parts(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_linear8_bias_of_another_type(device):
+    """16-bit weights beside a 32-bit bias: its gradient is not rounded to 16 bits."""
+    x = torch.randn(300, 40, device=device).to(torch.bfloat16)
+    w = torch.randn(24, 40, device=device).to(torch.bfloat16).requires_grad_()
+    b = torch.randn(24, device=device, requires_grad=True)
+    dy = torch.randn(300, 24, device=device).to(torch.bfloat16)
+    dw, db = torch.autograd.grad(linear8(x, w, b), (w, b), dy)
+    assert dw.dtype == torch.bfloat16 and db.dtype == torch.float32
+    d = dy.cpu().double()
+    close(db, d.sum(0), d.abs().sum(0), 300, "db")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_linear8_under_autocast(device):
     kind = torch.device(device).type
     x = torch.randn(20, 40, device=device, requires_grad=True)
@@ -399,3 +412,16 @@ def test_save8_beyond_32_bits():
     saved = save8(x)
     got = load8(saved)
     assert torch.equal(got[-7:].double().cpu(), kept8(tail)) and not got[:-7].any()
+
+
+@pytest.mark.gpu
+def test_weight_gradient_beyond_32_bits():
+    """More than 2^31 values of dy, and of codes."""
+    N, O, F = 2**20 + 3, 2080, 2080
+    dy = torch.zeros(N, O, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(N, F, dtype=torch.bfloat16, device="cuda")
+    dy[-7:], x[-7:] = torch.randn(7, O), torch.randn(7, F)
+    dw, db = weight_grad8(dy, save8(x), bias=True, dtype=torch.float32)
+    d, q = dy[-7:].cpu().double(), kept8(x[-7:])
+    close(dw, d.t() @ q, d.abs().t() @ q.abs(), 7, "dw")
+    close(db, d.sum(0), d.abs().sum(0), 7, "db")

@@ -380,6 +380,10 @@ def test_step_refuses():
         (9000, 37, 25),   # narrow rows, staged: runs at every 2-byte place
         (6000, 35, 50),
         (4500, 33, 33),   # a sequence a wave
+        (3, 9, 130),      # a wave walks alone, row by row
+        (2100, 40, 130),
+        (2100, 33, 65),
+        (4100, 21, 64),
     ],
 )
 def test_every_way_of_splitting(B, T, D, dtype, gate, keep):
