@@ -23,6 +23,7 @@ import numpy as np
 import torch
 
 from ..runtime.trainer import TrainHistory
+from .checkpoint8 import linear8
 
 logger = logging.getLogger(__name__)
 
@@ -39,17 +40,19 @@ def _packed_weights(module, device, dtype):
     return packed
 
 
-def _lstm_layer(x, w_ih_t, w_hh_t, b, H):
+def _lstm_layer(x, w_ih_t, w_hh_t, b, H, checkpoint8=False):
     """x [B,T,I] -> h_seq [B,T,H]: one x-projection GEMM for all timesteps,
     then per step one mm + ATen's fused differentiable LSTM cell (the same
     pointwise kernel torch.nn.LSTM uses on CUDA; dispatching it directly
-    bypasses the slow MIOpen RNN route on ROCm)."""
+    bypasses the slow MIOpen RNN route on ROCm). With ``checkpoint8`` the
+    projection keeps x as 8-bit codes, a quarter of its bytes."""
     B, T, I = x.shape
     # [T,B,4H] so each timestep slice is contiguous for the fused cell
-    gx = (
-        torch.addmm(b, x.reshape(-1, I), w_ih_t)
-        .view(B, T, 4 * H).transpose(0, 1).contiguous()
-    )
+    if checkpoint8:
+        gx = linear8(x, w_ih_t.t(), b)
+    else:
+        gx = torch.addmm(b, x.reshape(-1, I), w_ih_t)
+    gx = gx.view(B, T, 4 * H).transpose(0, 1).contiguous()
     h = x.new_zeros(B, H)
     c = x.new_zeros(B, H)
     outs = []
@@ -70,12 +73,12 @@ def _lstm_layer(x, w_ih_t, w_hh_t, b, H):
     return torch.stack(outs, dim=1)
 
 
-def wide_forward(module, x):
+def wide_forward(module, x, checkpoint8=False):
     """Full stacked forward: windows [B,T,F] -> head output [B,F_out]."""
     packed = _packed_weights(module, x.device, x.dtype)
     h = x
     for (w_ih_t, w_hh_t, b), cell in zip(packed, module.cells):
-        h = _lstm_layer(h, w_ih_t, w_hh_t, b, cell.hidden_size)
+        h = _lstm_layer(h, w_ih_t, w_hh_t, b, cell.hidden_size, checkpoint8)
     last = h[:, -1, :]
     return module.head_act(module.head(last))
 
@@ -114,7 +117,7 @@ class WideLSTMTrainer:
         # fp32 throughout: the step is kernel-count-bound, not GEMM-bound,
         # and the fused ATen cell is fp32-first
         def fwd_loss(w, tgt):
-            return loss_fn(wide_forward(module, w), tgt)
+            return loss_fn(wide_forward(module, w, getattr(cfg, "checkpoint8", False)), tgt)
 
         # ---- hipGraph capture of the whole fwd+bwd (static shapes) --------
         graph = None

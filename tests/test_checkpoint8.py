@@ -372,6 +372,41 @@ def test_block_trains(device):
         assert float((got - w).norm() / w.norm()) < 0.05
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_wide_lstm_keeps_its_inputs_in_8_bits(device):
+    """The wide-LSTM path under ``checkpoint8``: the same outputs, gradients near
+    the full ones, and no window in more than 8 bits between the two passes."""
+    from gordo_amd.model.factories.lstm_autoencoder import lstm_symmetric
+    from gordo_amd.ops.wide_lstm import wide_forward
+
+    module = lstm_symmetric(n_features=12, dims=[40], lookback_window=9).to(device)
+    w = torch.randn(6, 9, 12, device=device)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        out = wide_forward(module, w, checkpoint8=True)
+    full = wide_forward(module, w)
+    assert torch.allclose(out, full, atol=1e-5)
+    assert not any(t.is_floating_point() and t.numel() in (6 * 9 * 12, 6 * 9 * 40) for t in kept)
+    params = list(module.parameters())
+    got = torch.autograd.grad(out.square().mean(), params)
+    for g, f in zip(got, torch.autograd.grad(full.square().mean(), params)):
+        assert float((g - f).norm() / f.norm()) < 0.05  # a kept value is within 2^-7 of its group's largest
+
+
+@pytest.mark.gpu
+def test_wide_lstm_estimator_trains_from_8_bits():
+    """A width that no fused cell covers, from the estimator's own arguments, captured."""
+    import numpy as np
+
+    from gordo_amd.model.models import TorchLSTMAutoEncoder
+
+    X = np.random.default_rng(0).normal(size=(60, 10)).astype(np.float32)
+    model = TorchLSTMAutoEncoder(kind="lstm_symmetric", dims=[260], lookback_window=6, epochs=1, batch_size=16, seed=0, checkpoint8=True)
+    model.fit(X)
+    assert model.history["engine"] == "wide_lstm_gemmloop_graph"
+    assert np.isfinite(model.history["loss"]).all() and np.isfinite(model.predict(X)).all()
+
+
 @pytest.mark.gpu
 def test_linear8_captured():
     g = torch.Generator().manual_seed(4)
