@@ -24,6 +24,21 @@ struct alignas(16) C8Eight {
     typename E::store v[8];
 };
 
+// Eight values of a row of F from column `col` on, 0 behind the row. The hardware loads
+// and stores 16 bytes from any address of an element; only the eight at a row's end, if
+// it is short, goes value by value.
+template <class E>
+__device__ __forceinline__ C8Eight<E> c8_take(const typename E::store* row, int col, int F, bool in) {
+    C8Eight<E> v;
+    if (in && col + 8 <= F) {
+        __builtin_memcpy(&v, row + col, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = in && col + e < F ? row[col + e] : (typename E::store)0;
+    }
+    return v;
+}
+
 // VEC: rows start at 16-byte words and F is a multiple of 8
 template <class E, bool VEC>
 __global__ __launch_bounds__(256) void c8_save(const typename E::store* x, int64_t sx, signed char* codes,
@@ -39,15 +54,14 @@ __global__ __launch_bounds__(256) void c8_save(const typename E::store* x, int64
         const int64_t i = from + k * 256;
         row[k] = i < all ? i / each : 0;
         col[k] = i < all ? (int)(i - row[k] * each) * 8 : 0;
-        const typename E::store* at = x + row[k] * sx + col[k];
+        const typename E::store* at = x + row[k] * sx;
         if constexpr (VEC) {
-            if (i < all && col[k] < F) v[k] = *(const C8Eight<E>*)at;
+            if (i < all && col[k] < F) v[k] = *(const C8Eight<E>*)(at + col[k]);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[k].v[e] = 0;
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[k].v[e] = i < all && col[k] + e < F ? at[e] : (typename E::store)0;
+            v[k] = c8_take<E>(at, col[k], F, i < all);
         }
     }
 #pragma unroll
@@ -95,6 +109,8 @@ __global__ __launch_bounds__(256) void c8_load(const signed char* codes, const u
         typename E::store* at = x + row[k] * F + col[k];
         if constexpr (VEC) {
             *(C8Eight<E>*)at = v;
+        } else if (col[k] + 8 <= F) {
+            __builtin_memcpy(at, &v, sizeof(v));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -162,12 +178,6 @@ __device__ __forceinline__ c8_f32x4 wg_mfma(wg_s16x8 a, wg_s16x8 b, c8_f32x4 c) 
     if constexpr (std::is_same<E, C8Fp16>::value) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.f, y.f, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.h, y.h, c, 0, 0, 0);
 }
-
-// eight neighbouring values of a row of dy
-template <class E>
-struct WgEight {
-    typename E::store v[8];
-};
 
 // A buffer of the rows that are left, from this one on: what lies behind them reads as 0.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t wg_rows(const void* at, int64_t left, int64_t row_bytes) {
@@ -248,7 +258,7 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     // loads the scale of row i, and the others get it from there
     static_assert(NB <= 4, "a scale for each lane of a quad");
     const int os = fb8 < a.Fp ? (rb + (tid % NB) * RB) * ng + fb8 / C8_GROUP : WG_OUT;
-    WgEight<E> va[NA];
+    C8Eight<E> va[NA];
     uint2 vb[NB];
     int vs;
     auto load_a = [&](int i, int64_t n) {
@@ -260,11 +270,7 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
             for (int h = 0; h < ES / 2; ++h) to[h] = __builtin_amdgcn_raw_buffer_load_b128(rows, oa == WG_OUT ? WG_OUT : at + h * 16, 0, 0);
         } else {
             const int64_t row = n + ra + i * RA;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int o = o0 + ca * 8 + e;
-                va[i].v[e] = row < n1 && o < a.O ? dy[row * a.sdy + o] : (typename E::store)0;
-            }
+            va[i] = c8_take<E>(dy + row * a.sdy, o0 + ca * 8, a.O, row < n1);
         }
     };
     auto load_b = [&](int i, int64_t n) {
@@ -276,7 +282,7 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
     auto put_a = [&](int i, char* buf) {
         char* at = buf + wg_at(ra + i * RA, ca, PA);
         if constexpr (NP == 1) {
-            *(WgEight<E>*)at = va[i];
+            *(C8Eight<E>*)at = va[i];
         } else {
             float f[8];
 #pragma unroll
