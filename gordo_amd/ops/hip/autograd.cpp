@@ -69,10 +69,14 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     }
 };
 
+Tensor project(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias) {
+    const auto type = x.scalar_type();
+    return at::linear(x, weight.to(type), bias.has_value() ? c10::optional<Tensor>(bias->to(type)) : c10::nullopt);
+}
+
 struct Linear8 : torch::autograd::Function<Linear8> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias) {
-        const Tensor w = weight.to(x.scalar_type());
-        const Tensor y = at::linear(x, w, bias.has_value() ? c10::optional<Tensor>(bias->to(x.scalar_type())) : c10::nullopt);
+        const Tensor y = project(x, weight, bias);
         Tensor codes, scales;
         if (weight.requires_grad()) {
             const int64_t F = x.size(-1);
@@ -83,7 +87,6 @@ struct Linear8 : torch::autograd::Function<Linear8> {
         ctx->saved_data["x"] = x.requires_grad();
         ctx->saved_data["bias"] = bias.has_value() && bias->requires_grad();
         ctx->saved_data["bias_type"] = (int64_t)(bias.has_value() ? bias->scalar_type() : weight.scalar_type());
-        // float16 codes are exact in float16 only where the input was float16
         ctx->save_for_backward({weight, codes, scales});
         return y;
     }
@@ -123,5 +126,6 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor p, int64_t dim, c10::optional<Tenso
 
 Tensor linear8(Tensor x, Tensor weight, c10::optional<Tensor> bias) {
     c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+    if (!at::GradMode::is_enabled()) return project(x, weight, bias);
     return Linear8::apply(x, weight, bias);
 }

@@ -179,13 +179,14 @@ __device__ __forceinline__ c8_f32x4 wg_mfma(wg_s16x8 a, wg_s16x8 b, c8_f32x4 c) 
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.h, y.h, c, 0, 0, 0);
 }
 
+// an offset behind every buffer: for columns that do not exist (a tile's own are below 2^30)
+#define WG_OUT 0x7ffffff0
+
 // A buffer of the rows that are left, from this one on: what lies behind them reads as 0.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t wg_rows(const void* at, int64_t left, int64_t row_bytes) {
     const int64_t bytes = left > 0 ? left * row_bytes : 0;
-    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes < 0x7fffffff ? (int)bytes : 0x7fffffff, 0x00027000);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes < WG_OUT ? (int)bytes : WG_OUT, 0x00027000);
 }
-
-#define WG_OUT 0x7ffffff0  // an offset behind every buffer
 
 typedef unsigned int wg_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int wg_u32x2 __attribute__((ext_vector_type(2)));

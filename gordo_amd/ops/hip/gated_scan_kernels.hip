@@ -196,7 +196,7 @@ __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
 // workspace gives NaN and no hang.
 // ---------------------------------------------------------------------------
 #define GS_LB 16
-#define GS_SPINS (1 << 20)
+#define GS_SPINS (1 << 22)  // some seconds
 
 __device__ __forceinline__ unsigned int gs_word(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 
@@ -243,8 +243,9 @@ __device__ __forceinline__ void gs_place(const GsArgs& a, GsChain<V, W>& s, int&
 
 // The state that enters this wave's tile, from `carry` (the state that enters the
 // block's first tile; of the chain's first block where blocks are chained), and,
-// where a block walks on, in `carry` the state after its last tile. `mine`: this wave's map; `order`:
-// this wave's place in the block, 0 first. j counts tiles in the chain's order.
+// where a block walks on, in `carry` the state after its last tile. `mine`: this
+// wave's map; `order`: this wave's place in the block, 0 first. j counts tiles in the
+// chain's order.
 // `meanwhile` is done after this block's map is out and before others' are waited for.
 template <int V, int W, class F>
 __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int cg, int j, int order, int lane,
