@@ -57,8 +57,8 @@ struct GsPack {
 // A token behind its sequence's end: shut gate (r = +inf, so k = 0 and the state and
 // the gradient pass through), nothing in x and z. Whatever p holds there is gone
 // before it is used, and the loops over a tile need no masks.
-template <class E, int V, int P>
-__device__ __forceinline__ void gs_mask(GsPack<E, V> (&raw)[P][GS_R], int i, bool out) {
+template <class E, int V, int P, int R>
+__device__ __forceinline__ void gs_mask(GsPack<E, V> (&raw)[P][R], int i, bool out) {
     const unsigned int inf = sizeof(typename E::store) == 4 ? 0x7f800000u : (std::is_same<E, C8Bf16>::value ? 0x7f80u : 0x7c00u) * (V == 2 ? 0x10001u : 1u);
     raw[0][i].w = out ? 0u : raw[0][i].w;
     raw[1][i].w = out ? inf : raw[1][i].w;
@@ -98,7 +98,8 @@ struct GsArgs {
     // chained blocks (null: a block walks all its tiles)
     unsigned int* ticket;
     unsigned long long* agg;  // [nJ][groups][V][64]: a tile's (A, H), all ones until it is there
-    unsigned int* prefix;     // [nJ / GS_LB][groups][V][64]: state after a run of GS_LB tiles
+    unsigned int* prefix;     // [nJ / lb][groups][V][64]: state after a run of lb tiles
+    int lb;                   // tiles of a link
 };
 
 __device__ __forceinline__ int gs_len(const GsArgs& a, int b) {
@@ -182,10 +183,10 @@ __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
 //
 // With few channels, time is split over blocks too. Block j needs the state
 // after tile j - 1, and gets it without a second pass over the data: every block
-// publishes its (A, H) as soon as it has it, and every GS_LB-th block, which
-// folds the GS_LB - 1 before it, the state after itself. So a block reads at most
-// GS_LB words a channel, the serial chain has nJ / GS_LB links, and the order of
-// the folds is fixed: the same inputs give the same bits.
+// publishes its (A, H) as soon as it has it, and every LB-th block, which folds the
+// LB - 1 before it, the state after itself. So a block reads at most LB words a
+// channel, the serial chain has nJ / LB links of some 0.9 us, and the order of the
+// folds is fixed: the same inputs give the same bits.
 //
 // (A, H) is one 64-bit word, the prefix one 32-bit word: a word is there when it
 // is no longer all ones (a NaN is published as the canonical one), so data and
@@ -195,7 +196,7 @@ __device__ __forceinline__ GsLane gs_lane(const GsArgs& a, int64_t id) {
 // already: every wait ends. The bound on the spins is there so that a broken
 // workspace gives NaN and no hang.
 // ---------------------------------------------------------------------------
-#define GS_LB 16
+#define GS_LB 32  // tiles of a link at most
 #define GS_SPINS (1 << 22)  // some seconds
 
 __device__ __forceinline__ unsigned int gs_word(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
@@ -274,9 +275,9 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
             }
         }
     };
-    const int i = j % GS_LB, g = j / GS_LB;
+    const int lb = a.lb, i = j % lb, g = j / lb;
     const bool more = j + 1 < a.nJ;
-    if (a.ticket != nullptr && order == W - 1 && i < GS_LB - 1 && more) {
+    if (a.ticket != nullptr && order == W - 1 && i < lb - 1 && more) {
         parts();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -298,7 +299,7 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
     int spins = 0;
     for (int q = order; q < i; q += W) {
         unsigned long long word[V];
-        const unsigned long long* from = a.agg + ((int64_t)(g * GS_LB + q) * a.groups + cg) * V * 64 + lane;
+        const unsigned long long* from = a.agg + ((int64_t)(g * lb + q) * a.groups + cg) * V * 64 + lane;
         bool there;
         do {
             there = true;
@@ -338,7 +339,7 @@ __device__ __forceinline__ void gs_join(const GsArgs& a, GsChain<V, W>& s, int c
 #pragma unroll
             for (int v = 0; v < V; ++v) start[v] = __uint_as_float(word[v]);
         }
-        if (i == GS_LB - 1 && more) {
+        if (i == lb - 1 && more) {
 #pragma unroll
             for (int v = 0; v < V; ++v)
                 __hip_atomic_store(a.prefix + (((int64_t)g * a.groups + cg) * V + v) * 64 + lane,
@@ -363,14 +364,14 @@ __global__ __launch_bounds__(256) void gs_clear(uint4* to, int64_t n) {
 
 // The codes and scales of a tile of one part. The 32 values of a group are pairs
 // in 16 lanes (V = 2) or one in each of 32 (V = 1). A tile has 16 tokens: lane i of
-// 16 takes the largest magnitude of token i, so the scales of all tokens are made
+// 16 (fewer in a short one) takes the largest magnitude of token i, so the scales of all tokens are made
 // at once and stored once, and come back to the lanes by a broadcast.
-template <class E, int V>
-__device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&raw)[GS_R], bool live, bool mine, int64_t row,
+template <class E, int V, int R>
+__device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&raw)[R], bool live, bool mine, int64_t row,
                                           int64_t step, int64_t group, int left, int dd, int lane) {
     unsigned int top = 0;
 #pragma unroll
-    for (int i = 0; i < GS_R; ++i) {
+    for (int i = 0; i < R; ++i) {
         unsigned int t = c8_mag(raw[i].get(0));
         if constexpr (V == 2) t = max(t, c8_mag(raw[i].get(1)));
         t = c8_max16(live ? t : 0u);
@@ -380,7 +381,7 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
     const unsigned int scale = c8_scale(top);
     const float mine_inv = c8_inv(scale);
     signed char* to = a.codes + row * a.Dp + dd;
-    c8_for<GS_R>([&](auto n) {
+    c8_for<R>([&](auto n) {
         constexpr int i = decltype(n)::value;
         // row_newbcast: lane i's value to its 16 lanes
         const float inv = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(mine_inv), 0x150 + i, 0xF, 0xF, true));
@@ -397,7 +398,7 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
     if (mine && (V == 2 || (lane & 16) == 0)) a.scales[(group + dd / C8_GROUP) * GS_R + (lane & 15)] = (unsigned char)scale;
 }
 
-template <class E, int V, int P, bool KEEP, int W, bool STAGE = false>
+template <class E, int V, int P, bool KEEP, int W, bool STAGE = false, int R = GS_R>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(GsArgs a) {
     typedef GsPack<E, V> pack;
     static_assert(!STAGE || (W == 1 && V == 1), "staged: a wave alone, a channel a lane");
@@ -408,7 +409,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
     const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
-    const int nT = (a.T + GS_R - 1) / GS_R;
+    const int nT = (a.T + GS_R - 1) / GS_R;  // kept states
+    static_assert(R == GS_R || W == 1, "shorter tiles are for sequences of one tile");
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
     typename E::store* y = (typename E::store*)a.y + (int64_t)l.b * a.T * a.D + l.d;
 
@@ -422,49 +424,49 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
     const char* mine_p = nullptr;
     char* mine_y = nullptr;
     if constexpr (STAGE) {
-        // a tile is GS_R rows: its start within a word is the sequence's own, tile after tile
+        // a tile is R rows: its start within a word is the sequence's own, tile after tile
         mine_p = gs_lds + l.seq * a.pitch_p + (int)((uintptr_t)((const typename E::store*)a.p + l.b * a.sb) & 3) + l.d * ES;
         mine_y = lds_y + l.seq * a.pitch_y + (int)((uintptr_t)((const typename E::store*)a.y + (int64_t)l.b * a.T * a.D) & 3) + l.d * ES;
     }
     auto stage = [&](int tile) {
         for (int s = 0; s < a.seqs; ++s) {
-            const int64_t b = cg * (int64_t)a.seqs + s, t0 = (int64_t)tile * GS_R;
+            const int64_t b = cg * (int64_t)a.seqs + s, t0 = (int64_t)tile * R;
             if (b < a.B && t0 < a.T)
-                gs_stage_in((const char*)((const typename E::store*)a.p + b * a.sb + t0 * a.st), min(GS_R, a.T - (int)t0) * P * a.D * ES,
+                gs_stage_in((const char*)((const typename E::store*)a.p + b * a.sb + t0 * a.st), min(R, a.T - (int)t0) * P * a.D * ES,
                             gs_lds + s * a.pitch_p, lane);
         }
     };
     if constexpr (STAGE) stage(0);
 
     for (; j < end; ++j) {
-        const int tile = j * W + wid, t0 = tile * GS_R;
-        pack raw[P][GS_R];
+        const int tile = j * W + wid, t0 = tile * R;
+        pack raw[P][R];
         if constexpr (STAGE) {
             gs_staged();
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
                 for (int q = 0; q < P; ++q) raw[q][i].load((const typename E::store*)(mine_p + (i * P + q) * a.D * ES));
             gs_taken();
             stage(tile + 1);
         } else {
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
+            for (int i = 0; i < R; ++i) {
                 const int t = min(t0 + i, a.T - 1);
 #pragma unroll
                 for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
             }
         }
-        if (!__all(l.len >= t0 + GS_R)) {
+        if (!__all(l.len >= t0 + R)) {
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) gs_mask<E, V, P>(raw, i, t0 + i >= l.len);
+            for (int i = 0; i < R; ++i) gs_mask<E, V, P, R>(raw, i, t0 + i >= l.len);
         }
-        float k[GS_R][V], h[V];
+        float k[R][V], h[V];
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
+        for (int i = 0; i < R; ++i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 k[i][v] = gs_sigmoid(-raw[1][i].get(v));
@@ -485,8 +487,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
 #pragma unroll
-                    for (int i = 0; i < GS_R; ++i) raw[q][i].pin();
-                    gs_encode<E, V>(a, raw[q], l.live, kept && tile < nT, row + q, P, (((int64_t)l.b * nT + tile) * P + q) * (a.Dp / C8_GROUP), a.T - t0, dd, lane);
+                    for (int i = 0; i < R; ++i) raw[q][i].pin();
+                    gs_encode<E, V, R>(a, raw[q], l.live, kept && tile < nT, row + q, P, (((int64_t)l.b * nT + tile) * P + q) * (a.Dp / C8_GROUP), a.T - t0, dd, lane);
                 }
             }
         });
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
         }
 #pragma unroll
-        for (int i = 0; i < GS_R; ++i) {
+        for (int i = 0; i < R; ++i) {
             float out[V];
             raw[0][i].pin();
 #pragma unroll
@@ -520,14 +522,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             for (int s = 0; s < a.seqs; ++s) {
                 const int64_t b = cg * (int64_t)a.seqs + s;
                 if (b < a.B)
-                    gs_stage_out((char*)((typename E::store*)a.y + (b * a.T + t0) * a.D), min(GS_R, a.T - t0) * a.D * ES, lds_y + s * a.pitch_y, lane);
+                    gs_stage_out((char*)((typename E::store*)a.y + (b * a.T + t0) * a.D), min(R, a.T - t0) * a.D * ES, lds_y + s * a.pitch_y, lane);
             }
         } else if (l.live) {
             const float zero[V] = {};
-            for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
+            for (int t = max(t0, l.len); t < min(t0 + R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
         }
         // from the wave that has the last token: the same bits however far the batch is padded
-        if (l.live && tile == max(l.len - 1, 0) / GS_R) {
+        if (l.live && tile == max(l.len - 1, 0) / R) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = h[v];
         }
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 // The chain carries c, from the last tile to the first. Kept codes are decoded as
 // they are loaded, to bf16, in which they are exact.
 // ---------------------------------------------------------------------------
-template <class E, int V, int P, bool KEEP, int W, bool STAGE = false>
+template <class E, int V, int P, bool KEEP, int W, bool STAGE = false, int R = GS_R>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(GsArgs a) {
     typedef GsPack<E, V> pack;
     extern __shared__ __attribute__((aligned(16))) char gs_lds[];
@@ -557,7 +559,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
     const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
-    const int nT = (a.T + GS_R - 1) / GS_R;
+    const int nT = (a.T + GS_R - 1) / GS_R;  // kept states
+    static_assert(R == GS_R || W == 1, "shorter tiles are for sequences of one tile");
     const int64_t row0 = (int64_t)l.b * a.T;
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
     const typename E::store* dy = (const typename E::store*)a.dy + l.b * a.dsb + l.d;
@@ -581,7 +584,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
     }
     auto stage = [&](int tile) {
         if (tile < 0) return;
-        const int t0 = tile * GS_R, rows = min(GS_R, a.T - t0);
+        const int t0 = tile * R, rows = min(R, a.T - t0);
         for (int s = 0; s < a.seqs; ++s) {
             const int64_t b = cg * (int64_t)a.seqs + s;
             if (b >= a.B) break;
@@ -593,13 +596,13 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
     if constexpr (STAGE) stage(a.nJ - 1);
 
     for (; j < end; ++j) {
-        const int tile = (a.nJ - 1 - j) * W + wid, t0 = tile * GS_R;
-        GsPack<K, V> raw[P][GS_R];
-        pack up[GS_R];
+        const int tile = (a.nJ - 1 - j) * W + wid, t0 = tile * R;
+        GsPack<K, V> raw[P][R];
+        pack up[R];
         if constexpr (STAGE) {
             gs_staged();
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
+            for (int i = 0; i < R; ++i) {
                 up[i].load((const typename E::store*)(mine_dy + i * a.D * ES));
                 if constexpr (!KEEP)
 #pragma unroll
@@ -617,7 +620,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
 #pragma unroll
             for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[(group + (q * a.Dp + dd) / C8_GROUP) * GS_R + (lane & 15)]);
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
+            for (int i = 0; i < R; ++i) {
                 const int t = min(t0 + i, a.T - 1);
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
@@ -628,8 +631,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
             if constexpr (!STAGE)
 #pragma unroll
-                for (int i = 0; i < GS_R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
-            c8_for<GS_R>([&](auto n) {
+                for (int i = 0; i < R; ++i) up[i].load(dy + (int64_t)min(t0 + i, a.T - 1) * a.dst);
+            c8_for<R>([&](auto n) {
                 constexpr int i = decltype(n)::value;
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
@@ -644,7 +647,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             });
         } else if constexpr (!STAGE) {
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
+            for (int i = 0; i < R; ++i) {
                 const int t = min(t0 + i, a.T - 1);
                 up[i].load(dy + (int64_t)t * a.dst);
 #pragma unroll
@@ -654,19 +657,19 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = a.states[((int64_t)l.b * nT + min(tile, nT - 1)) * a.D + l.d + v];
-        if (!__all(l.len >= t0 + GS_R)) {
+        if (!__all(l.len >= t0 + R)) {
 #pragma unroll
-            for (int i = 0; i < GS_R; ++i) {
-                gs_mask<K, V, P>(raw, i, t0 + i >= l.len);
+            for (int i = 0; i < R; ++i) {
+                gs_mask<K, V, P, R>(raw, i, t0 + i >= l.len);
                 up[i].w = t0 + i >= l.len ? 0u : up[i].w;
             }
         }
-        float k[GS_R][V], c[V];
+        float k[R][V], c[V];
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
 #pragma unroll
-        for (int i = GS_R - 1; i >= 0; --i) {
+        for (int i = R - 1; i >= 0; --i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 k[i][v] = gs_sigmoid(-raw[1][i].get(v));
@@ -686,7 +689,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c, [] {});
         // the states of half a tile at a time: the first half's are computed twice
         // (two operations each), and half of them in registers is enough
-        constexpr int HALF = GS_R / 2;
+        constexpr int HALF = R / 2;
         float first[V], before[HALF][V];
 #pragma unroll
         for (int v = 0; v < V; ++v) first[v] = h[v];
@@ -752,11 +755,11 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             for (int s = 0; s < a.seqs; ++s) {
                 const int64_t b = cg * (int64_t)a.seqs + s;
                 if (b < a.B)
-                    gs_stage_out((char*)((typename E::store*)a.dp + (b * a.T + t0) * P * a.D), min(GS_R, a.T - t0) * P * a.D * ES, lds_dp + s * a.pitch_p, lane);
+                    gs_stage_out((char*)((typename E::store*)a.dp + (b * a.T + t0) * P * a.D), min(R, a.T - t0) * P * a.D * ES, lds_dp + s * a.pitch_p, lane);
             }
         } else if (l.live) {
             const float zero[V] = {};
-            for (int t = max(t0, l.len); t < min(t0 + GS_R, a.T); ++t)
+            for (int t = max(t0, l.len); t < min(t0 + R, a.T); ++t)
 #pragma unroll
                 for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)t * P + q) * a.D, zero);
         }
@@ -884,8 +887,10 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
 // Where a wave walks alone, narrow rows that are not whole sectors (64 bytes) go
 // through LDS: 8192 sequences of 144 tokens, 25 channels in bf16, take 53 + 75 us that way,
 // forward and backward, and 64 + 102 row by row.
+// Sequences of up to 4 tokens have tiles of 4 (32768 of one token, 1024 channels:
+// forward 221 us in tiles of 16, 113 in tiles of 4).
 struct GsPlan {
-    int W;
+    int W, R;
     unsigned int blocks;
     torch::Tensor space;
     bool staged;
@@ -897,25 +902,30 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
     const int64_t groups = ((int64_t)a.B * a.tps + 63) / 64;
     TORCH_CHECK(groups <= INT_MAX && a.T <= (1 << 30), "gated_scan: sizes of p out of range");
     plan.W = a.T <= GS_R || groups >= 2048 ? 1 : many;
+    plan.R = a.T <= 4 ? 4 : GS_R;
+    a.lb = 1;  // no chain
     const int es = (int)p.element_size(), lanes = a.codes != nullptr ? a.Dp : a.D;
     if (plan.W == 1 && a.D <= 64 && a.D * es % 64 != 0 && (a.T == 1 || (a.st == (int64_t)parts * a.D && (a.dy == nullptr || a.dst == a.D)))) {
         plan.staged = true;
         a.tps = lanes;
         a.seqs = 64 / lanes;
-        a.pitch_p = (GS_R * parts * a.D * es + 7) / 4 * 4;
-        a.pitch_y = (GS_R * a.D * es + 7) / 4 * 4;
-        a.nJ = (a.T + GS_R - 1) / GS_R;
+        a.pitch_p = (plan.R * parts * a.D * es + 7) / 4 * 4;
+        a.pitch_y = (plan.R * a.D * es + 7) / 4 * 4;
+        a.nJ = (a.T + plan.R - 1) / plan.R;
         plan.blocks = (unsigned int)((a.B + a.seqs - 1) / a.seqs);
         const int p_in = a.dy != nullptr && a.codes != nullptr ? 0 : a.pitch_p;
         plan.lds = (size_t)a.seqs * (p_in + a.pitch_y + (a.dy != nullptr ? a.pitch_p : 0));
         return plan;
     }
     a.groups = (int)groups;
-    a.nJ = (a.T + plan.W * GS_R - 1) / (plan.W * GS_R);
+    a.nJ = (a.T + plan.W * plan.R - 1) / (plan.W * plan.R);
     int64_t blocks = groups;
     if (plan.W > 1 && groups < 512 && a.nJ > 4) {
         blocks = groups * a.nJ;
-        const int64_t words = blocks * V * 64, links = (int64_t)((a.nJ + GS_LB - 1) / GS_LB) * groups * V * 64;
+        // Links of 16 tiles, where those take as long as a link by their bytes; else 32
+        // (1 sequence of 131072 tokens, 64 channels: 58 + 111 us in links of 16, 45 + 76 of 32).
+        a.lb = groups * plan.W * V < 32 ? GS_LB : 16;
+        const int64_t words = blocks * V * 64, links = (int64_t)((a.nJ + a.lb - 1) / a.lb) * groups * V * 64;
         const int64_t n = (words * 8 + links * 4 + 16 + 15) / 16;
         plan.space = torch::empty({n * 16}, p.options().dtype(at::kByte));
         char* at = (char*)plan.space.data_ptr();
@@ -935,7 +945,9 @@ struct GsFwdCall {
     hipStream_t stream;
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        if (plan.R == 4 && plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true, 4>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        else if (plan.R == 4) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        else if (plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
         else if (plan.W == 1) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, KEEP ? 4 : 8>), dim3(plan.blocks), dim3(KEEP ? 256 : 512), 0, stream, a);
     }
@@ -952,7 +964,9 @@ struct GsBwdCall {
     hipStream_t stream;
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        if (plan.R == 4 && plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true, 4>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        else if (plan.R == 4) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
+        else if (plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
         else if (plan.W == 1) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 4>), dim3(plan.blocks), dim3(256), 0, stream, a);
     }

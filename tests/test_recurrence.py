@@ -373,6 +373,10 @@ def test_step_refuses():
         (2, 5000, 33),    # many links, lanes that straddle two sequences
         (1, 4097, 1),     # one channel
         (5, 1100, 130),
+        (4, 2300, 200),   # links of 16 tiles, forward too
+        (3, 4, 130),      # short tiles
+        (50, 2, 64),
+        (40000, 1, 66),
         (700, 150, 50),   # a block walks several tiles
         (600, 650, 120),  # many of them
         (2200, 70, 62),   # a wave walks alone
