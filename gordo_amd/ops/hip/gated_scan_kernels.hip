@@ -799,37 +799,62 @@ __device__ __forceinline__ int64_t gs_slot(const GsStepArgs& a, int b) {
 template <class E, int V, int P>
 __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
     typedef GsPack<E, V> pack;
-    const int row = blockIdx.x;
+    __shared__ int found[4];
+    const int row = blockIdx.x, step = blockDim.x * V;
     const int64_t slot = a.slots != nullptr ? gs_slot(a, row) : row;
     typename E::store* y = (typename E::store*)a.y;
     if (slot < 0 || slot >= a.S) {  // no state: a row of padding
         const float zero[V] = {};
-        for (int d = threadIdx.x * V; d < a.D; d += blockDim.x * V) pack::put(y + (int64_t)row * a.D + d, zero);
+        for (int d = threadIdx.x * V; d < a.D; d += step) pack::put(y + (int64_t)row * a.D + d, zero);
         return;
+    }
+    pack raw[P];
+    float h[V];
+    auto load = [&](int b, int d) {
+        const typename E::store* p = (const typename E::store*)a.p + b * a.sb + d;
+#pragma unroll
+        for (int q = 0; q < P; ++q) raw[q].load(p + (int64_t)q * a.D);
+    };
+    auto state = [&](int d) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = a.state[slot * a.D + d + v];
+    };
+    int d = threadIdx.x * V;
+    if (d < a.D) {  // under way while the slots are looked through
+        load(row, d);
+        state(d);
     }
     int later = 0;
     if (a.slots != nullptr) {
-        int earlier = 0;
-        for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
-            if (b != row && gs_slot(a, b) == slot) {
-                earlier |= b < row;
-                later |= b > row;
+        int other = 0;  // 1: an earlier row has the slot, 2: a later one
+        auto look = [&](int b, int64_t s) {
+            if (s == slot && b != row) other |= b < row ? 1 : 2;
+        };
+        int from = 0;
+        if (!a.slots64 && ((uintptr_t)a.slots & 15) == 0) {  // four at a time
+            from = a.B & ~3;
+            for (int b = threadIdx.x * 4; b < from; b += blockDim.x * 4) {
+                const int4 four = *(const int4*)((const int*)a.slots + b);
+                look(b, four.x);
+                look(b + 1, four.y);
+                look(b + 2, four.z);
+                look(b + 3, four.w);
             }
         }
-        if (__syncthreads_or(earlier)) return;
-        later = __syncthreads_or(later);
+        for (int b = from + threadIdx.x; b < a.B; b += blockDim.x) look(b, gs_slot(a, b));
+        const int both = (__any(other & 1) ? 1 : 0) | (__any(other & 2) ? 2 : 0);
+        if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = both;
+        __syncthreads();
+        for (int w = 0; w < (int)blockDim.x >> 6; ++w) later |= found[w];
+        if (later & 1) return;
     }
-    for (int d = threadIdx.x * V; d < a.D; d += blockDim.x * V) {
-        float h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = a.state[slot * a.D + d + v];
-        for (int b = row; b < a.B; ++b) {
-            if (b != row && gs_slot(a, b) != slot) continue;
-            const typename E::store* p = (const typename E::store*)a.p + b * a.sb + d;
-            pack raw[P];
+    for (; d < a.D; d += step) {
+        if (d >= step) {
+            load(row, d);
+            state(d);
+        }
+        for (int b = row;;) {
             float out[V];
-#pragma unroll
-            for (int q = 0; q < P; ++q) raw[q].load(p + (int64_t)q * a.D);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 h[v] = fmaf(gs_sigmoid(-raw[1].get(v)), raw[0].get(v) - h[v], h[v]);
@@ -841,6 +866,10 @@ __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
             }
             pack::put(y + (int64_t)b * a.D + d, out);
             if (!later) break;
+            do ++b;
+            while (b < a.B && gs_slot(a, b) != slot);
+            if (b >= a.B) break;
+            load(b, d);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) a.out[slot * a.D + d + v] = h[v];

@@ -329,6 +329,31 @@ def test_slots(device, index, apart):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize("first", [0, 1])
+def test_many_rows_share_slots(device, index, first):
+    """Several tokens of many streams in one call, slots at any address: as token after token."""
+    B, S, D = 403, 150, 34
+    g = torch.Generator().manual_seed(8)
+    p = inputs(B, 1, D, torch.float32, "cpu")[0][:, 0]
+    slots = torch.randint(-5, S + 5, (B + first,), generator=g, dtype=index)[first:]
+    state = torch.randn(S, D, generator=g)
+    want, ys = state.double(), torch.zeros(B, D, dtype=torch.float64)
+    for b, s in enumerate(slots.tolist()):
+        if 0 <= s < S:
+            x, r, z = p[b].double().split(D)
+            want[s] = torch.sigmoid(r) * want[s] + torch.sigmoid(-r) * x
+            ys[b] = want[s] * z * torch.sigmoid(z)
+    on = slots.to(device)
+    if first:  # .to() makes a buffer of its own: put it at an odd place again
+        on = torch.cat([on[:first], on])[first:]
+    state = state.to(device)
+    y = gated_step(p.to(device), state, on)
+    near(y, ys, 25.0, 20, "y")
+    near(state, want, 5.0, 20, "state")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_step_of_nothing(device):
     state = torch.randn(3, 4, device=device)
     assert gated_step(torch.randn(0, 8, device=device), state, torch.zeros(0, dtype=torch.int32, device=device)).shape == (0, 4)
