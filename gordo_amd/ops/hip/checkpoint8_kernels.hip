@@ -194,13 +194,13 @@ typedef unsigned int wg_u32x2 __attribute__((ext_vector_type(2)));
 // eight codes and their scale as 16-bit numbers
 template <class E>
 __device__ __forceinline__ uint4 wg_decode(uint2 codes, unsigned int scale) {
-    const float s = c8_step(scale), off = -128.f * s;
+    const float s = c8_step(scale);
     unsigned int out[4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const unsigned int w = (h == 0 ? codes.x : codes.y) ^ 0x80808080u;  // code + 128, unsigned
-        const float f0 = fmaf((float)(w & 0xff), s, off), f1 = fmaf((float)((w >> 8) & 0xff), s, off);
-        const float f2 = fmaf((float)((w >> 16) & 0xff), s, off), f3 = fmaf((float)(w >> 24), s, off);
+        const unsigned int w = h == 0 ? codes.x : codes.y;
+        const float f0 = (float)(signed char)w * s, f1 = (float)(signed char)(w >> 8) * s;
+        const float f2 = (float)(signed char)(w >> 16) * s, f3 = (float)(signed char)(w >> 24) * s;
         if constexpr (std::is_same<E, C8Fp16>::value) {
             out[2 * h] = wg_pair(C8Fp16::down(f0), C8Fp16::down(f1));
             out[2 * h + 1] = wg_pair(C8Fp16::down(f2), C8Fp16::down(f3));
@@ -290,13 +290,14 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
             for (int e = 0; e < 8; ++e) f[e] = E::up(va[i].v[e]);
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
-                unsigned short h[8];
+                unsigned int w[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = C8Bf16::down(f[e]);
-                    f[e] -= C8Bf16::up(h[e]);
+                for (int e = 0; e < 8; e += 2) {  // cut, not rounded: a large finite number must not become infinite
+                    w[e / 2] = __builtin_amdgcn_perm(__float_as_uint(f[e + 1]), __float_as_uint(f[e]), 0x07060302u);
+                    f[e] -= __uint_as_float(w[e / 2] << 16);
+                    f[e + 1] -= __uint_as_float(w[e / 2] & 0xffff0000u);
                 }
-                *(uint4*)(at + q * SA) = uint4{wg_pair(h[0], h[1]), wg_pair(h[2], h[3]), wg_pair(h[4], h[5]), wg_pair(h[6], h[7])};
+                *(uint4*)(at + q * SA) = uint4{w[0], w[1], w[2], w[3]};
             }
         }
     };

@@ -197,6 +197,29 @@ def test_weight_gradient_of_values_beyond_float16(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_weight_gradient_of_the_largest_values(device, dtype):
+    """Inputs up to the largest finite number, whose steps are 2^121."""
+    g = torch.Generator().manual_seed(8)
+    x = (torch.rand(70, 40, generator=g) * 2 - 1) * torch.finfo(dtype).max
+    dy = torch.randn(70, 33, generator=g) * 2.0**-100
+    dw, _ = check_weight_grad(dy.to(dtype).to(device), x.to(dtype).to(device), torch.float32)
+    assert dw.isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_largest_32_bit_gradient(device):
+    """A finite gradient stays finite where the next bf16 number is infinite."""
+    top = torch.finfo(torch.float32).max
+    g = torch.Generator().manual_seed(9)
+    dy = torch.stack([torch.full((5,), top), torch.full((5,), -top)]).to(device)
+    x = (torch.randn(2, 40, generator=g) * 2.0**-100).to(device)
+    dw, db = check_weight_grad(dy, x, torch.float32)
+    assert dw.isfinite().all() and not db.any()
+    check_weight_grad(dy[:1], x[:1], torch.float32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("of_dy", DTYPES, ids=str)
 @pytest.mark.parametrize("to", DTYPES, ids=str)
 @pytest.mark.parametrize("N", [70, 3001])
@@ -435,6 +458,40 @@ def test_linear8_captured():
         torch.cuda.synchronize()
         for a, b_ in zip(out, want):
             assert torch.equal(a, b_)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("frozen", [False, True], ids=["32-bit bias", "frozen weight"])
+def test_linear8_bias_gradient_captured(frozen):
+    g = torch.Generator().manual_seed(10)
+    N, F, O = 5000, 70, 300
+    x, w, dy = (torch.randn(*s, generator=g).to(torch.bfloat16).cuda() for s in ((N, F), (O, F), (N, O)))
+    b = torch.randn(O, generator=g).cuda()
+
+    def work():
+        leaves = [t.detach().requires_grad_() for t in ((x, b) if frozen else (x, b, w))]
+        y = linear8(leaves[0], w if frozen else leaves[2], leaves[1])
+        return torch.autograd.grad(y, leaves, dy)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        work()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for _ in range(4):
+        for t in (x, dy):
+            t.copy_(torch.randn(t.shape, generator=g))
+        want = work()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b_ in zip(out, want):
+            assert torch.equal(a, b_)
+        d = dy.cpu().double()
+        close(out[1], d.sum(0), d.abs().sum(0), N, "db")
 
 
 @pytest.mark.gpu
