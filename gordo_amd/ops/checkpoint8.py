@@ -94,8 +94,11 @@ def _check_saved(saved: Saved8, what: str = "saved") -> int:
     """The row length of ``saved``; raises where its parts do not belong together."""
     if not isinstance(saved, Saved8):
         raise ValueError(f"{what} must be a Saved8, got {type(saved)}")
-    F = saved.shape[-1]
-    N, groups = saved.shape.numel() // F, -(-F // GROUP)
+    shape = torch.Size(saved.shape)
+    if len(shape) == 0 or shape[-1] == 0 or saved.dtype not in _DTYPES:
+        raise ValueError(f"{what}: no tensor of shape {tuple(shape)} and type {saved.dtype} is kept")
+    F = shape[-1]
+    N, groups = shape.numel() // F, -(-F // GROUP)
     if (saved.codes.shape != (N, groups * GROUP) or saved.scales.shape != (N, groups)
             or saved.codes.dtype != torch.int8 or saved.scales.dtype != torch.uint8
             or saved.codes.device != saved.scales.device

@@ -457,7 +457,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                 for (int q = 0; q < P; ++q) raw[q][i].load(p + (int64_t)t * a.st + q * a.D);
             }
         }
-        if (!__all(l.len >= t0 + R)) {
+        const bool whole = __all(l.len >= t0 + R);
+        if (!whole) {
 #pragma unroll
             for (int i = 0; i < R; ++i) gs_mask<E, V, P, R>(raw, i, t0 + i >= l.len);
         }
@@ -496,6 +497,26 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
             for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
         }
+        // h_last comes from the wave that has the last token: the same bits however far the
+        // batch is padded. A shut gate passes a state on, but not one that overflowed
+        // (0 times infinity): with padding in the tile, it is taken at its token.
+        const bool last = l.live && tile == max(l.len - 1, 0) / R;
+        if (!whole) {
+            float e[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) e[v] = h[v];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                raw[0][i].pin();
+#pragma unroll
+                for (int v = 0; v < V; ++v) e[v] = t0 + i < l.len ? fmaf(k[i][v], raw[0][i].get(v) - e[v], e[v]) : e[v];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (last) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = e[v];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float out[V];
@@ -528,8 +549,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             const float zero[V] = {};
             for (int t = max(t0, l.len); t < min(t0 + R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
         }
-        // from the wave that has the last token: the same bits however far the batch is padded
-        if (l.live && tile == max(l.len - 1, 0) / R) {
+        if (whole && last) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = h[v];
         }
@@ -1163,5 +1183,7 @@ torch::Tensor gated_step_launch(torch::Tensor p, torch::Tensor state, c10::optio
     GsStepCall call{a, threads, at::hip::getCurrentHIPStream().stream()};
     gs_types(p.scalar_type(), pair, p.size(1) / dim, call);
     C10_HIP_KERNEL_LAUNCH_CHECK();
+    // a graph that has kept what was in `out` is told that it changed
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return y;
 }

@@ -173,7 +173,7 @@ def gated_scan(
         p = p.contiguous()
     if p.is_cuda:
         return ext().gated_scan(p, dim, h0, lengths, keep == "int8")
-    return _GatedScan.apply(p, torch.zeros(B, dim) if h0 is None else h0, lengths, dim, keep == "int8")
+    return _GatedScan.apply(p, p.new_zeros((B, dim), dtype=torch.float32) if h0 is None else h0, lengths, dim, keep == "int8")
 
 
 def gated_step(

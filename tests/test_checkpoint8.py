@@ -124,6 +124,9 @@ def test_checkpoint_refuses():
         lambda: load8(Saved8(s.codes, s.scales, torch.Size([4, 70]), s.dtype)),
         lambda: load8(Saved8(s.codes[:3], s.scales, s.shape, s.dtype)),
         lambda: load8(Saved8(s.codes.float(), s.scales, s.shape, s.dtype)),
+        lambda: load8(Saved8(s.codes, s.scales, torch.Size([4, 0]), s.dtype)),
+        lambda: load8(Saved8(s.codes, s.scales, torch.Size([]), s.dtype)),
+        lambda: load8(Saved8(s.codes, s.scales, s.shape, torch.int8), torch.float32),
         lambda: weight_grad8(torch.randn(5, 3), s),
         lambda: weight_grad8(torch.randn(2, 2, 3), s),
         lambda: weight_grad8(torch.randn(4, 3).double(), s),

@@ -239,6 +239,46 @@ def test_extreme_gates(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,D", [(3, 6), (40, 6), (40, 130), (1500, 64)])
+def test_overflowed_state_passes_padding(device, T, D):
+    """An infinite state is what it is behind a sequence's last token, and so is a
+    start state where there is no token at all."""
+    inf = float("inf")
+    p = torch.zeros(3, T, 2 * D, device=device)
+    p[1, 1, :D] = inf  # the last token of this one
+    p[:, 2:] = float("nan")
+    h0 = torch.tensor([inf, 1.0, -2.0], device=device)[:, None].expand(3, D)
+    y, last = gated_scan(p, D, h0, torch.tensor([0, 2, 1], device=device))
+    assert (last[0] == inf).all() and (last[1] == inf).all() and (last[2] == -1.0).all()
+    assert not y[0].any() and (y[1, 0] == 0.5).all() and (y[1, 1] == inf).all() and not y[1, 2:].any()
+
+
+def test_default_types_are_not_asked():
+    p = torch.randn(2, 5, 12)
+    want = gated_scan(p, 4)
+    try:
+        torch.set_default_dtype(torch.float64)
+        got = gated_scan(p, 4)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_tells_graphs_that_the_state_changed(device):
+    state = torch.ones(2, 4, device=device)
+    w = torch.ones(2, 4, device=device, requires_grad=True)
+    kept = (state * w).sum()
+    with torch.no_grad():
+        gated_step(torch.randn(2, 12, device=device), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    with torch.inference_mode():
+        state = torch.ones(2, 4, device=device)
+        assert gated_step(torch.randn(2, 12, device=device), state).isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_empty(device):
     h0 = torch.randn(2, 3, device=device)
     y, last = gated_scan(torch.randn(2, 0, 9, device=device), 3, h0)
