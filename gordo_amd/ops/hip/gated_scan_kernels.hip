@@ -116,15 +116,16 @@ struct GsLane {
 };
 
 // staged: a wave has whole sequences
+template <int V>
 __device__ __forceinline__ GsLane gs_lane_staged(const GsArgs& a, int64_t cg, int lane) {
     GsLane l;
     l.seq = lane / a.tps;
-    l.d = lane - l.seq * a.tps;
+    l.d = (lane - l.seq * a.tps) * V;
     const int64_t b = cg * a.seqs + l.seq;
     l.live = l.seq < a.seqs && b < a.B && l.d < a.D;
     l.seq = min(l.seq, a.seqs - 1);
     l.b = (int)min(b, (int64_t)a.B - 1);
-    l.d = min(l.d, a.D - 1);
+    l.d = min(l.d, a.D - V);
     l.len = l.live ? gs_len(a, l.b) : a.T;
     return l;
 }
@@ -401,14 +402,14 @@ __device__ __forceinline__ void gs_encode(const GsArgs& a, const GsPack<E, V> (&
 template <class E, int V, int P, bool KEEP, int W, bool STAGE = false, int R = GS_R>
 __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(GsArgs a) {
     typedef GsPack<E, V> pack;
-    static_assert(!STAGE || (W == 1 && V == 1), "staged: a wave alone, a channel a lane");
+    static_assert(!STAGE || W == 1, "staged: a wave alone");
     extern __shared__ __attribute__((aligned(16))) char gs_lds[];
     __shared__ GsChain<V, W> chain;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes: scalar
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
-    const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
+    const GsLane l = STAGE ? gs_lane_staged<V>(a, cg, lane) : gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;  // kept states
     static_assert(R == GS_R || W == 1, "shorter tiles are for sequences of one tile");
     const typename E::store* p = (const typename E::store*)a.p + l.b * a.sb + l.d;
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             if constexpr (KEEP) {
                 const int64_t row = ((int64_t)l.b * a.T + t0) * P;
                 // channel, padding included, and whether it is one
-                const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
+                const int dd = (STAGE ? lane % a.tps : (int)(id % a.tps)) * V;
                 const bool kept = STAGE ? lane / a.tps < a.seqs && cg * (int64_t)a.seqs + lane / a.tps < a.B : id < (int64_t)a.B * a.tps;
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
@@ -531,7 +532,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                 }
             }
             if constexpr (STAGE) {
-                if (t0 + i >= l.len) out[0] = 0.f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) out[v] = t0 + i >= l.len ? 0.f : out[v];
                 if (l.live) pack::put((typename E::store*)(mine_y + i * a.D * ES), out);
             } else if (l.live && t0 + i < l.len) {
                 pack::put(y + (int64_t)(t0 + i) * a.D, out);
@@ -578,7 +580,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
     int cg, j, end;
     gs_place<V, W>(a, chain, cg, j, end);
     const int64_t id = (int64_t)cg * 64 + lane;
-    const GsLane l = STAGE ? gs_lane_staged(a, cg, lane) : gs_lane<V>(a, id);
+    const GsLane l = STAGE ? gs_lane_staged<V>(a, cg, lane) : gs_lane<V>(a, id);
     const int nT = (a.T + GS_R - 1) / GS_R;  // kept states
     static_assert(R == GS_R || W == 1, "shorter tiles are for sequences of one tile");
     const int64_t row0 = (int64_t)l.b * a.T;
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             float step[P];
             const int64_t group = ((int64_t)l.b * nT + min(tile, nT - 1)) * P * (a.Dp / C8_GROUP);
             // the group's lanes stay together, padding included
-            const int dd = STAGE ? lane % a.tps : (int)(id % a.tps) * V;
+            const int dd = (STAGE ? lane % a.tps : (int)(id % a.tps)) * V;
 #pragma unroll
             for (int q = 0; q < P; ++q) step[q] = c8_step(a.scales[(group + (q * a.Dp + dd) / C8_GROUP) * GS_R + (lane & 15)]);
 #pragma unroll
@@ -758,7 +760,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                 if constexpr (STAGE) {
 #pragma unroll
                     for (int q = 0; q < P; ++q) {
-                        if (t0 + i >= l.len) out[q][0] = 0.f;
+#pragma unroll
+                        for (int v = 0; v < V; ++v) out[q][v] = t0 + i >= l.len ? 0.f : out[q][v];
                         if (l.live) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), out[q]);
                     }
                 } else if (l.live && t0 + i < l.len) {
@@ -933,16 +936,22 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
 // and more than a few tiles, blocks are chained along time. Forward without codes
 // fits 128 registers a lane: blocks of 8 waves, 4 waves a SIMD. The codes and the
 // backward pass need up to 168: blocks of 4, 3 waves a SIMD.
-// Where a wave walks alone, narrow rows that are not whole sectors (64 bytes) go
+// Staging: where a wave walks alone, narrow rows that are not whole sectors (64 bytes) go
 // through LDS: 8192 sequences of 144 tokens, 25 channels in bf16, take 53 + 75 us that way,
-// forward and backward, and 64 + 102 row by row.
+// forward and backward, and 64 + 102 row by row. Rows of up to 64 channels have a lane for
+// each: more waves, more loads under way (144 tokens, 50 channels, x | r | z: 115 + 220 us,
+// 147 + 283 in pairs). In tiles of 4 tokens a wave has little to do, and pairs, which give
+// it two rows, are faster (200000 of 3 tokens, 50 channels: 85 + 133, and 115 + 154 a lane
+// each). Rows of 66 to 128 channels go in pairs (8192 x 144 x 70: 161 + 346, row by row 196
+// + 385), but not into codes (16384 x 40 x 100: 227 + 230, row by row 188 + 167) and not
+// in tiles of 4 (200000 x 3 x 100: 145 + 245, row by row 141 + 248).
 // Sequences of up to 4 tokens have tiles of 4 (32768 of one token, 1024 channels:
 // forward 221 us in tiles of 16, 113 in tiles of 4).
 struct GsPlan {
     int W, R;
     unsigned int blocks;
     torch::Tensor space;
-    bool staged;
+    int staged;  // channels of a lane, 0: not staged
     size_t lds;
 };
 
@@ -953,11 +962,14 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
     plan.W = a.T <= GS_R || groups >= 2048 ? 1 : many;
     plan.R = a.T <= 4 ? 4 : GS_R;
     a.lb = 1;  // no chain
-    const int es = (int)p.element_size(), lanes = a.codes != nullptr ? a.Dp : a.D;
-    if (plan.W == 1 && a.D <= 64 && a.D * es % 64 != 0 && (a.T == 1 || (a.st == (int64_t)parts * a.D && (a.dy == nullptr || a.dst == a.D)))) {
-        plan.staged = true;
-        a.tps = lanes;
-        a.seqs = 64 / lanes;
+    const int es = (int)p.element_size();
+    const bool narrow = a.D <= 64, brief = plan.R < GS_R;
+    const int stage = V == 2 && narrow == brief ? 2 : 1;
+    const bool fits = narrow || (a.D <= 128 && stage == 2 && a.codes == nullptr);
+    if (plan.W == 1 && fits && a.D * es % 64 != 0 && (a.T == 1 || (a.st == (int64_t)parts * a.D && (a.dy == nullptr || a.dst == a.D)))) {
+        plan.staged = stage;
+        a.tps = (a.codes != nullptr ? a.Dp : a.D) / stage;
+        a.seqs = 64 / a.tps;
         a.pitch_p = (plan.R * parts * a.D * es + 7) / 4 * 4;
         a.pitch_y = (plan.R * a.D * es + 7) / 4 * 4;
         a.nJ = (a.T + plan.R - 1) / plan.R;
@@ -992,11 +1004,21 @@ struct GsFwdCall {
     const GsArgs& a;
     const GsPlan& plan;
     hipStream_t stream;
+    void go(void (*staged)(GsArgs)) { hipLaunchKernelGGL(staged, dim3(plan.blocks), dim3(64), plan.lds, stream, a); }
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.R == 4 && plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true, 4>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
-        else if (plan.R == 4) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
-        else if (plan.staged) hipLaunchKernelGGL((gs_fwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        if (plan.staged) {
+            if constexpr (V == 2) {
+                if (plan.R == 4) go(gs_fwd<E, 2, P, KEEP, 1, true, 4>);
+                else if constexpr (!KEEP)
+                    if (plan.staged == 2) go(gs_fwd<E, 2, P, KEEP, 1, true>);
+            } else if (plan.R == 4) {
+                go(gs_fwd<E, 1, P, KEEP, 1, true, 4>);
+            }
+            if (plan.R == GS_R && plan.staged == 1) go(gs_fwd<E, 1, P, KEEP, 1, true>);
+            return;
+        }
+        if (plan.R == 4) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else if (plan.W == 1) hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_fwd<E, V, P, KEEP, KEEP ? 4 : 8>), dim3(plan.blocks), dim3(KEEP ? 256 : 512), 0, stream, a);
     }
@@ -1011,11 +1033,21 @@ struct GsBwdCall {
     const GsArgs& a;
     const GsPlan& plan;
     hipStream_t stream;
+    void go(void (*staged)(GsArgs)) { hipLaunchKernelGGL(staged, dim3(plan.blocks), dim3(64), plan.lds, stream, a); }
     template <class E, int V, int P, bool KEEP>
     void with() {
-        if (plan.R == 4 && plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true, 4>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
-        else if (plan.R == 4) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
-        else if (plan.staged) hipLaunchKernelGGL((gs_bwd<E, 1, P, KEEP, 1, true>), dim3(plan.blocks), dim3(64), plan.lds, stream, a);
+        if (plan.staged) {
+            if constexpr (V == 2) {
+                if (plan.R == 4) go(gs_bwd<E, 2, P, KEEP, 1, true, 4>);
+                else if constexpr (!KEEP)
+                    if (plan.staged == 2) go(gs_bwd<E, 2, P, KEEP, 1, true>);
+            } else if (plan.R == 4) {
+                go(gs_bwd<E, 1, P, KEEP, 1, true, 4>);
+            }
+            if (plan.R == GS_R && plan.staged == 1) go(gs_bwd<E, 1, P, KEEP, 1, true>);
+            return;
+        }
+        if (plan.R == 4) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1, false, 4>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else if (plan.W == 1) hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 1>), dim3(plan.blocks), dim3(64), 0, stream, a);
         else hipLaunchKernelGGL((gs_bwd<E, V, P, KEEP, 4>), dim3(plan.blocks), dim3(256), 0, stream, a);
     }

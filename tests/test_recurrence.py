@@ -463,6 +463,24 @@ def test_every_way_of_splitting(B, T, D, dtype, gate, keep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", [(7, 4, 2), (900, 3, 50), (5, 1, 62), (6, 11, 66), (3, 16, 126), (2700, 40, 100), (3, 2, 100)])
+def test_pairs_of_channels_in_narrow_rows(B, T, D, dtype, keep):
+    """16-bit rows that are whole words: as they lie, and with a word between sequences."""
+    p, h0, dy, dh = inputs(B, T, D, dtype, "cuda")
+    lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(3)).cuda()
+    a = check(p, D, h0, lengths, dy, dh, keep)
+    for first in (0, 1, 2):
+        n = T * 3 * D
+        buf = torch.full((B * (n + 2) + 2,), float("nan"), dtype=dtype, device="cuda")
+        view = buf.as_strided((B, T, 3 * D), (n + 2, 3 * D, 1), first)
+        view.copy_(p)
+        b = check(view, D, h0, lengths, dy, dh, keep)
+        assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("first", [0, 1, 2, 3])
 def test_narrow_rows_in_a_larger_buffer(first):
     """Dense sequences that start anywhere: what lies between them is left alone."""
