@@ -5,9 +5,10 @@
 //   h_t = h_{t-1} + k_t (x_t - h_{t-1})        ( = (1-k) h + k x )
 //   y_t = h_t * z_t * sigmoid(z_t)             (y_t = h_t without z)
 //
-// The update is written with k and not with 1 - k: a long memory has k near 0,
-// where 1 - k in 32 bits has lost k's digits. Every state is held in 32 bits;
-// only y and dp are rounded, once, to the type of p.
+// A long memory has k near 0, where 1 - k in 32 bits has lost k's digits; a token that
+// lets the state go has f = 1 - k near 0, where k has lost f's. So a gate is kept as the
+// smaller of the two, and which it is (gs_gate). Every state is held in 32 bits; only y and dp are
+// rounded, once, to the type of p.
 //
 // A wave owns 64 * V channels (V neighbours a lane) and takes GS_R tokens at a
 // time: all their loads are issued before the first is used, so that enough
@@ -25,6 +26,21 @@ namespace {
 __device__ __forceinline__ float gs_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 // exp overflows to +inf for x far below 0, whose reciprocal is the right 0
 __device__ __forceinline__ float gs_sigmoid(float x) { return gs_rcp(1.f + __expf(-x)); }
+
+// A gate of r in one register: the smaller of k = sigmoid(-r) and f = sigmoid(r), with all
+// its digits, as +k where r >= 0 and the state is held, as -f where it is let go. The
+// other one is 1 less the smaller, with all its digits too, and k f the product of both.
+__device__ __forceinline__ float gs_gate(float r) {
+    const float e = __expf(-fabsf(r));
+    return copysignf(e * gs_rcp(1.f + e), r);
+}
+__device__ __forceinline__ bool gs_holds(float gate) { return (int)__float_as_uint(gate) >= 0; }
+// k
+__device__ __forceinline__ float gs_takes(float gate) { return gs_holds(gate) ? gate : 1.f + gate; }
+// f v
+__device__ __forceinline__ float gs_passes(float gate, float v) { return fmaf(-gate, v, gs_holds(gate) ? v : 0.f); }
+// the state after a token
+__device__ __forceinline__ float gs_next(float gate, float x, float h) { return fmaf(gs_takes(gate), x - h, h); }
 
 // V neighbouring elements of type E as the register that a load fills. They stay
 // packed until they are used: 16-bit pairs as 32-bit floats would take twice the
@@ -463,7 +479,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
             for (int i = 0; i < R; ++i) gs_mask<E, V, P, R>(raw, i, t0 + i >= l.len);
         }
-        float k[R][V], h[V];
+        float gate[R][V], h[V];
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
@@ -471,10 +487,10 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
         for (int i = 0; i < R; ++i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                gate[i][v] = gs_gate(raw[1][i].get(v));
                 if constexpr (W > 1) {
-                    m[v].y = fmaf(k[i][v], raw[0][i].get(v) - m[v].y, m[v].y);
-                    m[v].x = fmaf(-k[i][v], m[v].x, m[v].x);
+                    m[v].y = gs_next(gate[i][v], raw[0][i].get(v), m[v].y);
+                    m[v].x = gs_passes(gate[i][v], m[v].x);
                 }
             }
             gs_fence<W>(i);
@@ -510,7 +526,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             for (int i = 0; i < R; ++i) {
                 raw[0][i].pin();
 #pragma unroll
-                for (int v = 0; v < V; ++v) e[v] = t0 + i < l.len ? fmaf(k[i][v], raw[0][i].get(v) - e[v], e[v]) : e[v];
+                for (int v = 0; v < V; ++v) e[v] = t0 + i < l.len ? gs_next(gate[i][v], raw[0][i].get(v), e[v]) : e[v];
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (last) {
@@ -524,7 +540,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             raw[0][i].pin();
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+                h[v] = gs_next(gate[i][v], raw[0][i].get(v), h[v]);
                 out[v] = h[v];
                 if constexpr (P == 3) {
                     const float z = raw[2][i].get(v);
@@ -565,8 +581,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 // ---------------------------------------------------------------------------
 // backward: tiles from the last to the first. The states of a tile are computed
 // again from the one kept before it, then
-//   g_t = dy_t silu(z_t) + c,  c = (1-k_t) g_t for the token before
-//   dx = g k, dr = g (h_{t-1} - x) k (1-k), dz = dy h silu'(z)
+//   g_t = dy_t silu(z_t) + c,  c = f_t g_t for the token before
+//   dx = g k, dr = g (h_{t-1} - x) k f, dz = dy h silu'(z)
 // The chain carries c, from the last tile to the first. Kept codes are decoded as
 // they are loaded, to bf16, in which they are exact.
 // ---------------------------------------------------------------------------
@@ -686,7 +702,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                 up[i].w = t0 + i >= l.len ? 0u : up[i].w;
             }
         }
-        float k[R][V], c[V];
+        float gate[R][V], c[V];
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
@@ -694,7 +710,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         for (int i = R - 1; i >= 0; --i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                k[i][v] = gs_sigmoid(-raw[1][i].get(v));
+                gate[i][v] = gs_gate(raw[1][i].get(v));
                 if constexpr (W > 1) {
                     float g = up[i].get(v);
                     if constexpr (P == 3) {
@@ -702,8 +718,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                         g *= z * gs_sigmoid(z);
                     }
                     g += m[v].y;
-                    m[v].y = fmaf(-k[i][v], g, g);
-                    m[v].x = fmaf(-k[i][v], m[v].x, m[v].x);
+                    m[v].y = gs_passes(gate[i][v], g);
+                    m[v].x = gs_passes(gate[i][v], m[v].x);
                 }
             }
             gs_fence<W>(i);
@@ -719,7 +735,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         for (int i = 0; i < HALF; ++i) {
             raw[0][i].pin();
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+            for (int v = 0; v < V; ++v) h[v] = gs_next(gate[i][v], raw[0][i].get(v), h[v]);
         }
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
@@ -730,7 +746,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     before[n][v] = h[v];
-                    h[v] = fmaf(k[i][v], raw[0][i].get(v) - h[v], h[v]);
+                    h[v] = gs_next(gate[i][v], raw[0][i].get(v), h[v]);
                 }
             }
             gs_fence<W>(0);
@@ -742,20 +758,19 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                 up[i].pin();
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float x = raw[0][i].get(v), kk = k[i][v], hp = before[n][v];
+                    const float x = raw[0][i].get(v), small = fabsf(gate[i][v]), hp = before[n][v];
                     float g = up[i].get(v);
                     if constexpr (P == 3) {
                         const float z = raw[2][i].get(v);
                         const float s = gs_sigmoid(z), zs = z * s;
-                        const float hn = fmaf(kk, x - hp, hp);
-                        out[2][v] = g * hn * fmaf(zs, 1.f - s, s);
+                        out[2][v] = g * (n == HALF - 1 ? h[v] : before[(n + 1) % HALF][v]) * fmaf(zs, 1.f - s, s);
                         g *= zs;
                     }
                     g += c[v];
-                    const float gk = g * kk;
-                    c[v] = g - gk;
-                    out[0][v] = gk;
-                    out[1][v] = (hp - x) * fmaf(-kk, gk, gk);
+                    const float less = small * g, more = fmaf(-small, g, g);  // k g and f g, or f g and k g
+                    c[v] = gs_holds(gate[i][v]) ? more : less;
+                    out[0][v] = gs_holds(gate[i][v]) ? less : more;
+                    out[1][v] = (hp - x) * (small * more);
                 }
                 if constexpr (STAGE) {
 #pragma unroll
@@ -880,7 +895,7 @@ __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
             float out[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = fmaf(gs_sigmoid(-raw[1].get(v)), raw[0].get(v) - h[v], h[v]);
+                h[v] = gs_next(gs_gate(raw[1].get(v)), raw[0].get(v), h[v]);
                 out[v] = h[v];
                 if constexpr (P == 3) {
                     const float z = raw[2].get(v);

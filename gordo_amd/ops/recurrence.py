@@ -37,18 +37,34 @@ def _live(T: int, lengths: Optional[torch.Tensor], device) -> Optional[torch.Ten
     return (torch.arange(T, device=device)[None] < lengths[:, None]).unsqueeze(-1)
 
 
+def _gate(r):
+    """(holds, small): the smaller of k = sigmoid(-r) and f = sigmoid(r), k where the
+    state is held (r >= 0). Either has all its digits that way; 1 - k near k = 1 has
+    lost those of f, 1 - f near f = 1 those of k. (From exp, whose bits do not depend on
+    a value's place in the tensor; torch.sigmoid's do, by the unit in the last place.)"""
+    e = torch.exp(-r.abs())
+    return r >= 0, e / (1 + e)
+
+
+def _next(gate, x, h):
+    """f h + k x"""
+    holds, small = gate
+    return h + torch.where(holds, small, 1 - small) * (x - h)
+
+
 def _scan_eager(p, dim, h0, live, start=None):
     """States before and after every token, float32. ``start``: the kept states,
     from which the recurrence goes on at every KEEP_EVERY-th token."""
     B, T = p.shape[:2]
-    x, k = p[..., :dim], torch.sigmoid(-p[..., dim : 2 * dim])
+    x = p[..., :dim]
+    holds, small = _gate(p[..., dim : 2 * dim])
     h = h0
     before, after = torch.empty_like(x), torch.empty_like(x)
     for t in range(T):
         if start is not None and t % KEEP_EVERY == 0:
             h = start[:, t // KEEP_EVERY]
         before[:, t] = h
-        n = h + k[:, t] * (x[:, t] - h)
+        n = _next((holds[:, t], small[:, t]), x[:, t], h)
         h = n if live is None else torch.where(live[:, t], n, h)
         after[:, t] = h
     return before, after, h
@@ -70,7 +86,8 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
     """p in float32 as it was kept."""
     live = _live(p.shape[1], lengths, p.device)
     before, after, _ = _scan_eager(p, dim, None, live, states)
-    x, k = p[..., :dim], torch.sigmoid(-p[..., dim : 2 * dim])
+    x = p[..., :dim]
+    holds, small = _gate(p[..., dim : 2 * dim])
     g, dp = dy.float(), torch.empty_like(p)
     if p.shape[2] == 3 * dim:
         z = p[..., 2 * dim :]
@@ -80,9 +97,11 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
     c = dh
     for t in range(p.shape[1] - 1, -1, -1):
         gt = g[:, t] + c
-        dp[:, t, :dim] = gt * k[:, t]
-        dp[:, t, dim : 2 * dim] = gt * (before[:, t] - x[:, t]) * k[:, t] * (1 - k[:, t])
-        n = gt * (1 - k[:, t])
+        less = small[:, t] * gt
+        more = gt - less
+        dp[:, t, :dim] = torch.where(holds[:, t], less, more)
+        dp[:, t, dim : 2 * dim] = (before[:, t] - x[:, t]) * (small[:, t] * more)
+        n = torch.where(holds[:, t], more, less)
         c = n if live is None else torch.where(live[:, t], n, c)
     if live is not None:
         dp = torch.where(live, dp, torch.zeros_like(dp))
@@ -231,7 +250,7 @@ def gated_step(
             y[b] = 0
             continue
         h = new.get(s, state[s])
-        h = h + torch.sigmoid(-pf[b, dim : 2 * dim]) * (pf[b, :dim] - h)
+        h = _next(_gate(pf[b, dim : 2 * dim]), pf[b, :dim], h)
         new[s] = h
         y[b] = h * torch.nn.functional.silu(pf[b, 2 * dim :]) if p.shape[1] == 3 * dim else h
     for s, h in new.items():

@@ -582,3 +582,50 @@ def test_offsets_beyond_32_bits():
     view.copy_(p)
     a, b = check(view, D, h0, None, dy, dh), check(p, D, h0, None, dy, dh)
     assert torch.equal(a[0], b[0]) and torch.equal(a[2][0], b[2][0])
+
+
+# ------------------------------------------ the digits of gates that hold and let go
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [37, 74, 1480])
+def test_gates_keep_their_digits_at_both_ends(device, D):
+    """f near 0 as k near 0: 1 - k has lost f's digits at r = -8, all of them at -18.
+
+    One token, so every output is a product: dx = g k, dr = g (h0 - x) k f, dh0 = g f,
+    and y = f h0 where x is 0. A gate is off by 2^-19 of itself (an argument of exp of
+    up to 18 log2(e) = 26 is rounded by 2^-20, times log 2; exp, 1 + e, the reciprocal
+    and the product some 2^-22 each), a product of two by twice that."""
+    r = torch.linspace(-18, 18, 37).repeat(D // 37)
+    x, h0 = torch.zeros(D), torch.full((D,), 3.0)
+    p = torch.cat([x, r])[None, None].to(device).requires_grad_()
+    h = h0[None].to(device).requires_grad_()
+    y, last = gated_scan(p, D, h)
+    dp, dh0 = torch.autograd.grad(last, (p, h), torch.full((1, D), 0.75, device=device))
+    f, k = torch.sigmoid(r.double()), torch.sigmoid(-r.double())
+
+    def relative(got, want, allowed):
+        off = (got.detach().cpu().double().flatten() / want - 1).abs()
+        assert float(off.max()) < allowed, (float(r[off.argmax()]), float(off.max()))
+
+    relative(dh0, 0.75 * f, 2.0**-19)
+    relative(dp[..., :D], 0.75 * k, 2.0**-19)
+    relative(dp[..., D:], 0.75 * 3 * k * f, 2.0**-18)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,D", [(5, 33), (40, 37), (40, 130), (300, 74), (1500, 37)])
+def test_one_token_lets_a_long_memory_go(device, T, D):
+    """All gates hold but one, at another token for each channel: what passes is f of
+    that one, also through the maps of tiles that are folded into each other."""
+    r = torch.full((T, D), 30.0)  # f = 1 - 2^-43
+    at = torch.randint(0, T, (D,), generator=torch.Generator().manual_seed(4))
+    lets = torch.linspace(-18, -8, D)
+    r[at, torch.arange(D)] = lets
+    p = torch.cat([torch.zeros(T, D), r], 1)[None].to(device).requires_grad_()
+    h = torch.full((1, D), 3.0, device=device, requires_grad=True)
+    y, last = gated_scan(p, D, h)
+    dp, dh0 = torch.autograd.grad(last, (p, h), torch.ones(1, D, device=device))
+    f = torch.sigmoid(lets.double())
+    # the other gates' products round to what they were: f of 1 - 2^-43 takes nothing away
+    assert float((dh0[0].cpu().double() / f - 1).abs().max()) < 2.0**-19
+    dr = dp[0, at, D + torch.arange(D)].cpu().double()
+    assert float((dr / (3 * f * (1 - f)) - 1).abs().max()) < 2.0**-18
