@@ -16,6 +16,8 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <cfloat>
+
 #include "checkpoint8.h"
 #include "launchers.h"
 
@@ -34,13 +36,16 @@ __device__ __forceinline__ float gs_gate(float r) {
     const float e = __expf(-fabsf(r));
     return copysignf(e * gs_rcp(1.f + e), r);
 }
-__device__ __forceinline__ bool gs_holds(float gate) { return (int)__float_as_uint(gate) >= 0; }
-// k
-__device__ __forceinline__ float gs_takes(float gate) { return gs_holds(gate) ? gate : 1.f + gate; }
+// where the gate holds, else lets go
+__device__ __forceinline__ float gs_pick(float gate, float holds, float lets_go) { return (int)__float_as_uint(gate) >= 0 ? holds : lets_go; }
 // f v
-__device__ __forceinline__ float gs_passes(float gate, float v) { return fmaf(-gate, v, gs_holds(gate) ? v : 0.f); }
-// the state after a token
-__device__ __forceinline__ float gs_next(float gate, float x, float h) { return fmaf(gs_takes(gate), x - h, h); }
+__device__ __forceinline__ float gs_passes(float gate, float v) { return fmaf(-gate, v, gs_pick(gate, v, 0.f)); }
+// the state after a token, as two products: x - h may be more than the largest number
+__device__ __forceinline__ float gs_next(float& gate, float x, float h) {
+    asm("" : "+v"(gate));  // what was made of it before is made anew: kept, it takes registers
+    const float most = gs_pick(gate, h, x), rest = gs_pick(gate, x, h), small = fabsf(gate);
+    return fmaf(small, rest, fmaf(-small, most, most));
+}
 
 // V neighbouring elements of type E as the register that a load fills. They stay
 // packed until they are used: 16-bit pairs as 32-bit floats would take twice the
@@ -86,6 +91,17 @@ __device__ __forceinline__ void gs_mask(GsPack<E, V> (&raw)[P][R], int i, bool o
 template <int W>
 __device__ __forceinline__ void gs_fence(int i) {
     if (W > 1 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+}
+
+// The gates of a tile's tokens.
+template <int W, class E, int V, int R>
+__device__ __forceinline__ void gs_gates(const GsPack<E, V> (&r)[R], float (&gate)[R][V]) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) gate[i][v] = gs_gate(r[i].get(v));
+        gs_fence<W>(i);
+    }
 }
 
 struct GsArgs {
@@ -483,17 +499,17 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+        if constexpr (W > 1) {
+            gs_gates<W>(raw[1], gate);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
+            for (int i = 0; i < R; ++i) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gate[i][v] = gs_gate(raw[1][i].get(v));
-                if constexpr (W > 1) {
+                for (int v = 0; v < V; ++v) {
                     m[v].y = gs_next(gate[i][v], raw[0][i].get(v), m[v].y);
                     m[v].x = gs_passes(gate[i][v], m[v].x);
                 }
+                gs_fence<W>(i);
             }
-            gs_fence<W>(i);
         }
         // the codes are made while the state is on its way
         gs_join<V, W>(a, chain, cg, j, wid, lane, m, carry, h, [&] {
@@ -510,6 +526,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                 }
             }
         });
+        if constexpr (W == 1) gs_gates<W>(raw[1], gate);  // here: packed, r takes fewer registers
         if (a.states != nullptr && l.live && tile < nT) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
@@ -703,45 +720,46 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
         }
         float gate[R][V], c[V];
+        gs_gates<W>(raw[1], gate);
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
+        if constexpr (W > 1) {
 #pragma unroll
-        for (int i = R - 1; i >= 0; --i) {
+            for (int i = R - 1; i >= 0; --i) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gate[i][v] = gs_gate(raw[1][i].get(v));
-                if constexpr (W > 1) {
+                for (int v = 0; v < V; ++v) {
                     float g = up[i].get(v);
                     if constexpr (P == 3) {
                         const float z = raw[2][i].get(v);
                         g *= z * gs_sigmoid(z);
                     }
-                    g += m[v].y;
-                    m[v].y = gs_passes(gate[i][v], g);
+                    m[v].y = gs_passes(gate[i][v], g + m[v].y);
                     m[v].x = gs_passes(gate[i][v], m[v].x);
                 }
+                gs_fence<W>(i);
             }
-            gs_fence<W>(i);
         }
         gs_join<V, W>(a, chain, cg, j, W - 1 - wid, lane, m, carry, c, [] {});
-        // the states of half a tile at a time: the first half's are computed twice
-        // (two operations each), and half of them in registers is enough
-        constexpr int HALF = R / 2;
-        float first[V], before[HALF][V];
+        // Beside other waves, and where codes take registers too, the states of half a tile at
+        // a time: the first half's are computed twice. A wave alone keeps all of them (8192
+        // sequences of 144 tokens, 70 channels: 356 us, in halves 384; 25 channels as codes,
+        // where all of them cost a wave a SIMD: 142, in halves 112).
+        constexpr int SPAN = W == 1 && !KEEP ? R : R / 2;
+        float first[V], before[SPAN][V];
 #pragma unroll
         for (int v = 0; v < V; ++v) first[v] = h[v];
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) {
+        for (int i = 0; i < R - SPAN; ++i) {
             raw[0][i].pin();
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = gs_next(gate[i][v], raw[0][i].get(v), h[v]);
         }
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
+        for (int half = R / SPAN - 1; half >= 0; --half) {
 #pragma unroll
-            for (int n = 0; n < HALF; ++n) {
-                const int i = half * HALF + n;
+            for (int n = 0; n < SPAN; ++n) {
+                const int i = half * SPAN + n;
                 raw[0][i].pin();
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -751,26 +769,27 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
             gs_fence<W>(0);
 #pragma unroll
-            for (int n = HALF - 1; n >= 0; --n) {
-                const int i = half * HALF + n;
+            for (int n = SPAN - 1; n >= 0; --n) {
+                const int i = half * SPAN + n;
                 float out[P][V];
                 raw[P - 1][i].pin();
                 up[i].pin();
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
+                    asm("" : "+v"(gate[i][v]));
                     const float x = raw[0][i].get(v), small = fabsf(gate[i][v]), hp = before[n][v];
                     float g = up[i].get(v);
                     if constexpr (P == 3) {
                         const float z = raw[2][i].get(v);
                         const float s = gs_sigmoid(z), zs = z * s;
-                        out[2][v] = g * (n == HALF - 1 ? h[v] : before[(n + 1) % HALF][v]) * fmaf(zs, 1.f - s, s);
+                        out[2][v] = g * fmaf(zs, 1.f - s, s) * (n == SPAN - 1 ? h[v] : before[(n + 1) % SPAN][v]);
                         g *= zs;
                     }
                     g += c[v];
                     const float less = small * g, more = fmaf(-small, g, g);  // k g and f g, or f g and k g
-                    c[v] = gs_holds(gate[i][v]) ? more : less;
-                    out[0][v] = gs_holds(gate[i][v]) ? less : more;
-                    out[1][v] = (hp - x) * (small * more);
+                    c[v] = gs_pick(gate[i][v], more, less);
+                    out[0][v] = gs_pick(gate[i][v], less, more);
+                    out[1][v] = fmaf(small, hp, -(small * x)) * more;  // small is at most 1/2: the difference does not overflow
                 }
                 if constexpr (STAGE) {
 #pragma unroll
@@ -895,7 +914,8 @@ __global__ __launch_bounds__(256) void gs_step(GsStepArgs a) {
             float out[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = gs_next(gs_gate(raw[1].get(v)), raw[0].get(v), h[v]);
+                float gate = gs_gate(raw[1].get(v));
+                h[v] = gs_next(gate, raw[0].get(v), h[v]);
                 out[v] = h[v];
                 if constexpr (P == 3) {
                     const float z = raw[2].get(v);

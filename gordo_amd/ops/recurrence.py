@@ -47,9 +47,10 @@ def _gate(r):
 
 
 def _next(gate, x, h):
-    """f h + k x"""
+    """f h + k x, as two products: x - h may be more than the largest number."""
     holds, small = gate
-    return h + torch.where(holds, small, 1 - small) * (x - h)
+    most, rest = torch.where(holds, h, x), torch.where(holds, x, h)
+    return (most - small * most) + small * rest
 
 
 def _scan_eager(p, dim, h0, live, start=None):
@@ -92,7 +93,7 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
     if p.shape[2] == 3 * dim:
         z = p[..., 2 * dim :]
         s = torch.sigmoid(z)
-        dp[..., 2 * dim :] = g * after * s * (1 + z * (1 - s))
+        dp[..., 2 * dim :] = g * (s * (1 + z * (1 - s))) * after
         g = g * z * s
     c = dh
     for t in range(p.shape[1] - 1, -1, -1):
@@ -100,7 +101,7 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
         less = small[:, t] * gt
         more = gt - less
         dp[:, t, :dim] = torch.where(holds[:, t], less, more)
-        dp[:, t, dim : 2 * dim] = (before[:, t] - x[:, t]) * (small[:, t] * more)
+        dp[:, t, dim : 2 * dim] = (small[:, t] * before[:, t] - small[:, t] * x[:, t]) * more
         n = torch.where(holds[:, t], more, less)
         c = n if live is None else torch.where(live[:, t], n, c)
     if live is not None:

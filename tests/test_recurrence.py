@@ -629,3 +629,59 @@ def test_one_token_lets_a_long_memory_go(device, T, D):
     assert float((dh0[0].cpu().double() / f - 1).abs().max()) < 2.0**-19
     dr = dp[0, at, D + torch.arange(D)].cpu().double()
     assert float((dr / (3 * f * (1 - f)) - 1).abs().max()) < 2.0**-18
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,D", [(1, 37), (1, 74), (40, 37), (300, 74)])
+def test_a_state_keeps_the_digits_of_what_is_let_go(device, T, D):
+    """x = 0 throughout: a state is the product of the f before it, whatever their size."""
+    r = torch.full((T, D), 30.0)
+    lets = torch.linspace(-18, 18, 37).repeat(D // 37)
+    r[T // 2] = lets
+    p = torch.cat([torch.zeros(T, D), r], 1)[None].to(device)
+    h0 = torch.full((1, D), 3.0, device=device)
+    y, last = gated_scan(p, D, h0)
+    want = 3 * torch.sigmoid(lets.double())
+    assert float((last[0].cpu().double() / want - 1).abs().max()) < 2.0**-19
+    assert torch.equal(y[0, -1], last[0])
+    gated_step(p[:, T // 2], h0)
+    assert float((h0[0].cpu().double() / want - 1).abs().max()) < 2.0**-19
+
+
+# ------------------------------------------------------------- near the largest number
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("B,T,D", [(3, 1, 40), (2, 2, 66), (3, 40, 33), (2, 700, 64), (1, 40, 130)])
+def test_states_between_the_largest_numbers(device, dtype, B, T, D):
+    """x and h of opposite signs, further apart than the largest number: a state lies
+    between them, and so does everything that is made of finite ones."""
+    g = torch.Generator().manual_seed(5)
+    top = torch.finfo(dtype).max
+    x = (torch.rand(B, T, D, generator=g) * 2 - 1) * top
+    x[:, ::3] = top
+    x[:, 1::3] = -top
+    p = torch.cat([x, torch.randn(B, T, D, generator=g) * 4], -1).to(dtype)
+    h0 = ((torch.rand(B, D, generator=g) * 2 - 1) * torch.finfo(torch.float32).max)
+    dy, dh = torch.randn(B, T, D, generator=g) * 2.0**-10, torch.randn(B, D, generator=g) * 2.0**-10
+    dy = dy.to(dtype)
+    want = definition(p, D, h0, None, dy, dh)
+    p, h0 = p.to(device).requires_grad_(), h0.to(device).requires_grad_()
+    y, last = gated_scan(p, D, h0)
+    dp, dh0 = torch.autograd.grad((y, last), (p, h0), (dy.to(device), dh.to(device)))
+    big = torch.finfo(torch.float32).max
+    near(y, want[0], big, T, "y")
+    near(last, want[1], big, T, "h_last")
+    near(dp[..., D:], want[2][..., D:], big * float(want[3].abs().max() + want[2][..., :D].abs().max()), T, "dr")
+    near(dh0, want[3], 0.1, T, "dh0")
+    state = h0.detach().clone()
+    with torch.no_grad():
+        near(gated_step(p[:, 0], state), want[0][:, 0], big, 1, "y of a step")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_opposite_values_meet_half_way(device):
+    x = torch.tensor([3e38, -3e38], device=device)
+    p = torch.stack([x, torch.zeros_like(x)], 1)[None]
+    y, last = gated_scan(p, 1)
+    # half of 3e38 is 1.5e38, half of that and half of -3e38: -7.5e37, two roundings each
+    assert abs(float(last) / -7.5e37 - 1) < 2.0**-20
