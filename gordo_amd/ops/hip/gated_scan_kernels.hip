@@ -75,15 +75,13 @@ struct GsPack {
     }
 };
 
-// A token behind its sequence's end: shut gate (r = +inf, so k = 0 and the state and
-// the gradient pass through), nothing in x and z. Whatever p holds there is gone
-// before it is used, and the loops over a tile need no masks.
+// A token behind its sequence's end: whatever p holds there is gone before it is used, and
+// its gate is f = 1 as such, which passes every state and gradient on as it is (an infinite
+// one too: 1 less a share of 0 would be no number). The loops over a tile need no masks.
 template <class E, int V, int P, int R>
 __device__ __forceinline__ void gs_mask(GsPack<E, V> (&raw)[P][R], int i, bool out) {
-    const unsigned int inf = sizeof(typename E::store) == 4 ? 0x7f800000u : (std::is_same<E, C8Bf16>::value ? 0x7f80u : 0x7c00u) * (V == 2 ? 0x10001u : 1u);
-    raw[0][i].w = out ? 0u : raw[0][i].w;
-    raw[1][i].w = out ? inf : raw[1][i].w;
-    if constexpr (P == 3) raw[2][i].w = out ? 0u : raw[2][i].w;
+#pragma unroll
+    for (int q = 0; q < P; ++q) raw[q][i].w = out ? 0u : raw[q][i].w;
 }
 
 // Where waves share a CU by registers, a scheduler that interleaves many tokens to
@@ -93,14 +91,20 @@ __device__ __forceinline__ void gs_fence(int i) {
     if (W > 1 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
 }
 
-// The gates of a tile's tokens.
+// The gates of a tile's tokens. whole: no token of the wave's lanes is behind its end.
 template <int W, class E, int V, int R>
-__device__ __forceinline__ void gs_gates(const GsPack<E, V> (&r)[R], float (&gate)[R][V]) {
+__device__ __forceinline__ void gs_gates(const GsPack<E, V> (&r)[R], float (&gate)[R][V], bool whole, int t0, int len) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
 #pragma unroll
         for (int v = 0; v < V; ++v) gate[i][v] = gs_gate(r[i].get(v));
         gs_fence<W>(i);
+    }
+    if (!whole) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) gate[i][v] = t0 + i >= len ? -1.f : gate[i][v];
     }
 }
 
@@ -500,7 +504,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
         if constexpr (W > 1) {
-            gs_gates<W>(raw[1], gate);
+            gs_gates<W>(raw[1], gate, whole, t0, l.len);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
 #pragma unroll
@@ -526,31 +530,14 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                 }
             }
         });
-        if constexpr (W == 1) gs_gates<W>(raw[1], gate);  // here: packed, r takes fewer registers
+        if constexpr (W == 1) gs_gates<W>(raw[1], gate, whole, t0, l.len);  // here: packed, r takes fewer registers
         if (a.states != nullptr && l.live && tile < nT) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.states[((int64_t)l.b * nT + tile) * a.D + l.d + v] = h[v];
         }
-        // h_last comes from the wave that has the last token: the same bits however far the
-        // batch is padded. A shut gate passes a state on, but not one that overflowed
-        // (0 times infinity): with padding in the tile, it is taken at its token.
+        // h_last comes from the wave that has the last token: what is behind it in its tile
+        // is padding, which passes the state on
         const bool last = l.live && tile == max(l.len - 1, 0) / R;
-        if (!whole) {
-            float e[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) e[v] = h[v];
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                raw[0][i].pin();
-#pragma unroll
-                for (int v = 0; v < V; ++v) e[v] = t0 + i < l.len ? gs_next(gate[i][v], raw[0][i].get(v), e[v]) : e[v];
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (last) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = e[v];
-            }
-        }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float out[V];
@@ -584,7 +571,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
             const float zero[V] = {};
             for (int t = max(t0, l.len); t < min(t0 + R, a.T); ++t) pack::put(y + (int64_t)t * a.D, zero);
         }
-        if (whole && last) {
+        if (last) {
 #pragma unroll
             for (int v = 0; v < V; ++v) a.h_last[(int64_t)l.b * a.D + l.d + v] = h[v];
         }
@@ -603,8 +590,10 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
 // The chain carries c, from the last tile to the first. Kept codes are decoded as
 // they are loaded, to bf16, in which they are exact.
 // ---------------------------------------------------------------------------
+// A lane of one 16-bit channel fits 128 registers: held to it, four waves a SIMD (with codes,
+// 8192 sequences of 144 tokens, 25 channels: 112 us, with a few registers more 140).
 template <class E, int V, int P, bool KEEP, int W, bool STAGE = false, int R = GS_R>
-__global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(GsArgs a) {
+__global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::store) == 2 ? 4 : 2) : W == 4 ? 3 : 4) void gs_bwd(GsArgs a) {
     typedef GsPack<E, V> pack;
     extern __shared__ __attribute__((aligned(16))) char gs_lds[];
     typedef typename std::conditional<KEEP, C8Bf16, E>::type K;  // type of the kept projection in registers
@@ -712,7 +701,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = a.states[((int64_t)l.b * nT + min(tile, nT - 1)) * a.D + l.d + v];
-        if (!__all(l.len >= t0 + R)) {
+        const bool whole = __all(l.len >= t0 + R);
+        if (!whole) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 gs_mask<K, V, P, R>(raw, i, t0 + i >= l.len);
@@ -720,7 +710,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
             }
         }
         float gate[R][V], c[V];
-        gs_gates<W>(raw[1], gate);
+        gs_gates<W>(raw[1], gate, whole, t0, l.len);
         float2 m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = float2{1.f, 0.f};
@@ -786,7 +776,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_bwd(Gs
                         g *= zs;
                     }
                     g += c[v];
-                    const float less = small * g, more = fmaf(-small, g, g);  // k g and f g, or f g and k g
+                    // k g and f g, or f g and k g. An infinite g stays so: 1 less a share is more than 0.
+                    const float less = small * g, more = fmaf(-small, __builtin_amdgcn_fmed3f(g, -FLT_MAX, FLT_MAX), g);
                     c[v] = gs_pick(gate[i][v], more, less);
                     out[0][v] = gs_pick(gate[i][v], less, more);
                     out[1][v] = fmaf(small, hp, -(small * x)) * more;  // small is at most 1/2: the difference does not overflow

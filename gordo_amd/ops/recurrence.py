@@ -28,6 +28,7 @@ from . import ext
 from .checkpoint8 import _DTYPES, codes_eager, first_order, values_eager
 
 KEEP_EVERY = 16  # tokens between two kept states
+_TOP = torch.finfo(torch.float32).max
 
 
 # ------------------------------------------------------------------ plain torch
@@ -99,7 +100,7 @@ def _backward_eager(p, dim, lengths, states, dy, dh):
     for t in range(p.shape[1] - 1, -1, -1):
         gt = g[:, t] + c
         less = small[:, t] * gt
-        more = gt - less
+        more = gt - small[:, t] * gt.clamp(-_TOP, _TOP)  # an infinite gradient stays so: 1 less a share is more than 0
         dp[:, t, :dim] = torch.where(holds[:, t], less, more)
         dp[:, t, dim : 2 * dim] = (small[:, t] * before[:, t] - small[:, t] * x[:, t]) * more
         n = torch.where(holds[:, t], more, less)

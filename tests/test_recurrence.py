@@ -685,3 +685,49 @@ def test_opposite_values_meet_half_way(device):
     y, last = gated_scan(p, 1)
     # half of 3e38 is 1.5e38, half of that and half of -3e38: -7.5e37, two roundings each
     assert abs(float(last) / -7.5e37 - 1) < 2.0**-20
+
+
+# ------------------------------------------------------------------ infinite gradients
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "plain"])
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("T,D", [(3, 6), (40, 6), (40, 130), (300, 64), (1500, 64)])
+def test_an_infinite_gradient_passes_padding(device, gate, keep, T, D):
+    """A gradient that a scaled loss has overflowed is what it is in front of the padding,
+    and is not taken for a number at the tokens before."""
+    inf = float("inf")
+    parts = 3 if gate else 2
+    p = torch.zeros(4, T, parts * D, device=device)
+    p[:, 2:] = float("nan")
+    dh = torch.tensor([inf, -inf, inf, 1.0], device=device)[:, None].expand(4, D).contiguous()
+    dy = torch.zeros(4, T, D, device=device)
+    dy[3, 2:] = inf
+    lengths = torch.tensor([0, 1, 2, 2], device=device)
+    p.requires_grad_()
+    h0 = torch.ones(4, D, device=device, requires_grad=True)
+    dp, dh0 = torch.autograd.grad(gated_scan(p, D, h0, lengths, keep=keep), (p, h0), (dy, dh))
+    # half gates: f = k = 1/2 at every token there is
+    assert (dh0[0] == inf).all() and (dh0[1] == -inf).all() and (dh0[2] == inf).all() and (dh0[3] == 0.25).all()
+    assert not dp[0].any() and not dp[1, 1:].any() and not dp[2:, 2:].any()
+    assert (dp[1, 0, :D] == -inf).all() and (dp[2, :2, :D] == inf).all()
+    assert (dp[3, :2, :D] == torch.tensor([0.25, 0.5], device=device)[:, None]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("B,T,D", [(2, 50, 20), (1, 50, 130), (1, 1200, 64)])
+def test_what_follows_no_number_is_none(device, bad, B, T, D):
+    """A state, or a gradient, that is not finite reaches all that depends on it."""
+    p, h0, dy, dh = inputs(B, T, D, torch.float32, device, gate=False)
+    at = T // 2
+    q = p.clone()
+    q[:, at, 3] = bad
+    y, last = gated_scan(q, D, h0)
+    assert not y[:, at:, 3].isfinite().any() and not last[:, 3].isfinite().any()
+    assert y[:, :at].isfinite().all() and y[..., 4:].isfinite().all()
+    dy[:, at, 3] = bad
+    p.requires_grad_()
+    h0.requires_grad_()
+    dp, dh0 = torch.autograd.grad(gated_scan(p, D, h0), (p, h0), (dy, dh))
+    assert not dp[:, : at + 1, 3].isfinite().any() and not dh0[:, 3].isfinite().any()
+    assert dp[:, at + 1 :].isfinite().all() and dp[..., 4:D].isfinite().all()
