@@ -22,6 +22,8 @@ void first_order(const char* what) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient has no gradient of its own (create_graph)");
 }
 
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 struct Scan {
     Tensor y, last, states, codes, scales;
 };
@@ -116,6 +118,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
 }  // namespace
 
 std::tuple<Tensor, Tensor> gated_scan(Tensor p, int64_t dim, c10::optional<Tensor> h0, c10::optional<Tensor> lengths, bool keep8) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(p) && !(h0.has_value() && dual(*h0)), "gated_scan: no forward mode (jvp)");
     if (at::GradMode::is_enabled() && (p.requires_grad() || (h0.has_value() && h0->requires_grad()))) {
         auto out = GatedScan::apply(p, h0, lengths, dim, keep8);
         return {out[0], out[1]};

@@ -1209,6 +1209,7 @@ void gated_scan_bwd_launch(torch::Tensor p, int64_t dim, c10::optional<torch::Te
 torch::Tensor gated_step_launch(torch::Tensor p, torch::Tensor state, c10::optional<torch::Tensor> slots,
                                 torch::Tensor out) {
     TORCH_CHECK(state.dim() == 2, "gated_step: state must be [slots, dim]");
+    for (const auto& t : {p, state, out}) TORCH_CHECK_VALUE(!t._fw_grad(/*level=*/0).defined(), "gated_step has no gradient, no forward mode either");
     const int64_t dim = state.size(1);
     TORCH_CHECK(p.is_cuda() && p.dim() == 2 && p.stride(1) == 1 && dim > 0 &&
                     (p.size(1) == 2 * dim || p.size(1) == 3 * dim) && p.size(0) > 0 && p.size(0) <= INT_MAX && p.size(1) <= INT_MAX,

@@ -173,7 +173,11 @@ def gated_scan(
              and takes the gradient at the kept values. States are kept in 32
              bits before every 16th token either way and computed again between.
 
-    y has the type of p, h_last is float32. Gradients: p and h0.
+    y has the type of p, h_last is float32. Gradients: p and h0, once, in reverse
+    mode; forward mode and gradients of gradients are refused.
+
+    A value that is not finite reaches all that depends on it, as one that is not
+    finite; whether it is infinite or no number may depend on how time is split.
     """
     _check_projection(p, dim, 3, "[B, T, parts * dim]")
     B, T = p.shape[:2]
@@ -217,7 +221,8 @@ def gated_step(
            shape that does not overlap it; slots that no row names are left as
            they are there.
 
-    It has no gradient (use :func:`gated_scan`), and refuses inputs that ask for one.
+    It has no gradient (use :func:`gated_scan`), and refuses inputs that ask for one,
+    forward mode's among them.
     """
     if not isinstance(state, torch.Tensor) or state.dtype != torch.float32 or state.dim() != 2 or not state.is_contiguous():
         raise ValueError("state must be contiguous float32 [slots, dim]")
@@ -243,6 +248,9 @@ def gated_step(
             raise ValueError("out overlaps state: pass state itself, or a buffer of its own")
     if B and p.is_cuda:
         return ext().gated_step(p if p.stride(1) == 1 else p.contiguous(), state, slots, out)
+    for t in (p, state, out):
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("gated_step has no gradient, no forward mode either")
     y = torch.empty((B, dim), dtype=p.dtype, device=p.device)
     pf = p.detach().float()
     new = {}

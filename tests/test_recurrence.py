@@ -731,3 +731,37 @@ def test_what_follows_no_number_is_none(device, bad, B, T, D):
     dp, dh0 = torch.autograd.grad(gated_scan(p, D, h0), (p, h0), (dy, dh))
     assert not dp[:, : at + 1, 3].isfinite().any() and not dh0[:, 3].isfinite().any()
     assert dp[:, at + 1 :].isfinite().all() and dp[..., 4:D].isfinite().all()
+
+
+# ---------------------------------------------------------------- calls with no answer
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_is_refused(device):
+    """A tangent is not dropped without a word: with and without gradients, of p and of h0."""
+    fw = torch.autograd.forward_ad
+    p, h0 = torch.randn(1, 4, 6, device=device), torch.randn(1, 3, device=device)
+    with fw.dual_level():
+        dual_p, dual_h = fw.make_dual(p, torch.ones_like(p)), fw.make_dual(h0, torch.ones_like(h0))
+        for call in (lambda: gated_scan(dual_p, 3), lambda: gated_scan(p, 3, dual_h),
+                     lambda: gated_scan(p.clone().requires_grad_(), 3, dual_h)):
+            with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+                call()
+            with torch.no_grad(), pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+                call()
+    assert gated_scan(p, 3, h0)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_refuses_tangents(device):
+    fw = torch.autograd.forward_ad
+    p, state = torch.randn(2, 9, device=device), torch.randn(2, 3, device=device)
+    kept = state.clone()
+    with fw.dual_level():
+        for make in (lambda: (fw.make_dual(p, torch.ones_like(p)), state, None),
+                     lambda: (p, fw.make_dual(state, torch.ones_like(state)), None),
+                     lambda: (p, state, fw.make_dual(state.clone(), torch.ones_like(state)))):
+            q, s, out = make()
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="no gradient"):
+                    gated_step(q, s, out=out)
+    assert torch.equal(state, kept)
+    gated_step(p, state)
