@@ -230,7 +230,7 @@ def gated_step(
     _check_projection(p, dim, 2, "[B, parts * dim]")
     if state.device != p.device:
         raise ValueError(f"state is on {state.device}, p on {p.device}")
-    if torch.is_grad_enabled() and (p.requires_grad or state.requires_grad):
+    if torch.is_grad_enabled() and (p.requires_grad or state.requires_grad or getattr(out, "requires_grad", False)):
         raise ValueError("gated_step has no gradient: call it under torch.no_grad()")
     B = p.shape[0]
     if slots is not None:

@@ -765,3 +765,18 @@ def test_step_refuses_tangents(device):
                     gated_step(q, s, out=out)
     assert torch.equal(state, kept)
     gated_step(p, state)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_refuses_an_out_that_asks_for_a_gradient(device):
+    """Overwritten in place, `out` would leave a graph with gradients of values that are gone."""
+    p, state = torch.randn(2, 9, device=device), torch.randn(2, 3, device=device)
+    w = torch.ones(2, 3, device=device, requires_grad=True)
+    part, leaf = w * 2, torch.zeros(2, 3, device=device, requires_grad=True)
+    for out in (part, leaf):
+        kept = out.detach().clone()
+        with pytest.raises(ValueError, match="no gradient"):
+            gated_step(p, state, out=out)
+        assert torch.equal(out, kept)
+    with torch.no_grad():
+        assert gated_step(p, state, out=leaf).isfinite().all() and leaf.any()
