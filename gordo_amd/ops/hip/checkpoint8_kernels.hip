@@ -179,6 +179,10 @@ __device__ __forceinline__ c8_f32x4 wg_mfma(wg_s16x8 a, wg_s16x8 b, c8_f32x4 c) 
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.h, y.h, c, 0, 0, 0);
 }
 
+// What is left of a number after its first piece: of an infinite one nothing. A NaN stays
+// one, also where its bits are all in the lower half and the piece is infinite.
+__device__ __forceinline__ float wg_rest(float f, float piece) { return __builtin_isinf(f) ? 0.f : f - piece; }
+
 // an offset behind every buffer: for columns that do not exist (a tile's own are below 2^30)
 #define WG_OUT 0x7ffffff0
 
@@ -294,8 +298,8 @@ __global__ __launch_bounds__(WG_THREADS, 2) void c8_weight_grad(WgArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {  // cut, not rounded: a large finite number must not become infinite
                     w[e / 2] = __builtin_amdgcn_perm(__float_as_uint(f[e + 1]), __float_as_uint(f[e]), 0x07060302u);
-                    f[e] -= __uint_as_float(w[e / 2] << 16);
-                    f[e + 1] -= __uint_as_float(w[e / 2] & 0xffff0000u);
+                    f[e] = wg_rest(f[e], __uint_as_float(w[e / 2] << 16));
+                    f[e + 1] = wg_rest(f[e + 1], __uint_as_float(w[e / 2] & 0xffff0000u));
                 }
                 *(uint4*)(at + q * SA) = uint4{w[0], w[1], w[2], w[3]};
             }

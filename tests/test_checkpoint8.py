@@ -520,3 +520,28 @@ def test_weight_gradient_beyond_32_bits():
     d, q = dy[-7:].cpu().double(), kept8(x[-7:])
     close(dw, d.t() @ q, d.abs().t() @ q.abs(), 7, "dw")
     close(db, d.sum(0), d.abs().sum(0), 7, "db")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N", [70, 3001])
+def test_weight_gradient_of_infinite_dy(device, dtype, N):
+    """What a scaled loss has overflowed to: infinite sums are infinite, of the sign that they
+    have, in 32 bits as in 16; a NaN of any bits is none."""
+    inf = float("inf")
+    dy = torch.randn(N, 20).to(dtype)
+    x = torch.rand(N, 40) + 0.5
+    dy[5, 1], dy[9, 2], dy[60, 3] = inf, -inf, float("nan")
+    dy[5, 4], dy[9, 4] = inf, -inf
+    if dtype == torch.float32:
+        dy[7, 6] = torch.tensor(0x7F800001, dtype=torch.int32).view(torch.float32)  # in its low half alone
+    dy, x = dy.to(device), x.to(dtype).to(device)
+    dw, db = weight_grad8(dy, save8(x), bias=True)
+    for got in (dw, db[:, None]):
+        assert (got[1] == inf).all() and (got[2] == -inf).all() and got[3].isnan().all() and got[4].isnan().all()
+        assert got[0].isfinite().all() and got[7:].isfinite().all()
+        assert got[6].isnan().all() if dtype == torch.float32 else got[6].isfinite().all()
+    b = torch.zeros(20, dtype=dtype, device=device, requires_grad=True)
+    w = torch.randn(20, 40, device=device).to(dtype)
+    frozen = torch.autograd.grad(linear8(x, w, b), b, dy)[0]
+    assert same(frozen.isfinite().float(), db.isfinite().float()) and (frozen[1] == inf).all()
