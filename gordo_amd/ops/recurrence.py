@@ -176,6 +176,9 @@ def gated_scan(
     y has the type of p, h_last is float32. Gradients: p and h0, once, in reverse
     mode; forward mode and gradients of gradients are refused.
 
+    The same call gives the same bits each time. A sequence's last bits may depend on
+    how time is split, which follows from the sizes of the call, padding included.
+
     A value that is not finite reaches all that depends on it, as one that is not
     finite; whether it is infinite or no number may depend on how time is split.
     """

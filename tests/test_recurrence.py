@@ -780,3 +780,30 @@ def test_step_refuses_an_out_that_asks_for_a_gradient(device):
         assert torch.equal(out, kept)
     with torch.no_grad():
         assert gated_step(p, state, out=leaf).isfinite().all() and leaf.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", ["input", "int8"])
+def test_bits_under_more_padding(keep):
+    """How time is split follows from the padded length: where the split is the same, so are
+    the bits; across its border (four tiles of 128 tokens in a block's walk, five and more
+    in a chain of blocks) a sequence's results are near."""
+    n, D = 500, 40
+    p, h0, dy, dh = inputs(2, n, D, torch.float32, "cuda")
+    want = definition(p, D, h0, None, dy, dh, keep)
+    runs = {}
+    for T in (n, 512, 513, 600, 640, 3000):
+        wide = torch.full((2, T, 3 * D), float("nan"), device="cuda")
+        wide_dy = torch.full((2, T, D), float("nan"), device="cuda")
+        wide[:, :n], wide_dy[:, :n] = p, dy
+        wide.requires_grad_()
+        h = h0.clone().requires_grad_()
+        y, last = gated_scan(wide, D, h, torch.full((2,), n, device="cuda"), keep=keep)
+        dp, dh0 = torch.autograd.grad((y, last), (wide, h), (wide_dy, dh))
+        runs[T] = y.detach()[:, :n], last.detach(), dp[:, :n], dh0
+        m = float(p.abs().max())
+        near(y[:, :n], want[0], m * m, n, "y")
+        near(last, want[1], m, n, "h_last")
+        near(dh0, want[3], 8.0, n, "dh0")
+    for a, b in ((n, 512), (513, 600), (600, 640)):
+        assert all(torch.equal(s, t) for s, t in zip(runs[a][:2], runs[b][:2]))
