@@ -807,3 +807,159 @@ def test_bits_under_more_padding(keep):
         near(dh0, want[3], 8.0, n, "dh0")
     for a, b in ((n, 512), (513, 600), (600, 640)):
         assert all(torch.equal(s, t) for s, t in zip(runs[a][:2], runs[b][:2]))
+
+
+# --------------------------------------------------- every element by its own error bound
+U = 2.0**-22  # four roundings of 2^-24: two of a token's update, two of the maps it goes through
+GATE = 2.0**-20  # a gate's smaller factor, relative: exp and reciprocal of an argument below 16
+
+
+def bounded(p, dim, h0, lengths, dy, dh, keep="input", seam=None):
+    """((value, error) of y, h_last, dp and dh0): the definition beside the first-order errors
+    of 32-bit arithmetic, token by token. M is a sum of magnitudes, E the error that it may
+    carry; both fade with the gates, so a bound is as local as the memory. What is in it:
+
+    - the smaller of f and k is off by GATE of itself, the other one by the same amount
+    - a token's update of a state, or of the gradient's carry, by U of its magnitudes
+    - silu by 2^-19 of itself (sigmoid 2^-20, products), silu' by 2^-18 of its two terms
+    - products and differences of these by their factors' errors and U of their magnitudes
+
+    ``seam``: the carry is lost in front of this token (a mistake for the test of the test)."""
+    p, dy, dh = (t.detach().cpu().double() for t in (p, dy, dh))
+    B, T, width = p.shape
+    h = torch.zeros(B, dim, dtype=torch.float64) if h0 is None else h0.detach().cpu().double()
+    n = torch.full((B, 1), T) if lengths is None else lengths.cpu().long().clamp(0, T)[:, None]
+    q = p if keep == "input" else torch.cat([kept8(part) for part in p.split(dim, -1)], -1)
+
+    def gates(p, t):
+        r = p[:, t, dim : 2 * dim]
+        return p[:, t, :dim], torch.sigmoid(r), torch.sigmoid(-r)
+
+    def token(p, t, h, M, E):
+        x, f, k = gates(p, t)
+        live = t < n
+        m = f * M + k * x.abs()
+        e = f * E + GATE * torch.minimum(f, k) * (x.abs() + M) + U * m
+        return torch.where(live, f * h + k * x, h), torch.where(live, m, M), torch.where(live, e, E)
+
+    def gate_of(p, t):
+        z = p[:, t, 2 * dim :]
+        s = torch.sigmoid(z)
+        return z, s, z * s
+
+    y, ey = torch.zeros(2, B, T, dim, dtype=torch.float64)
+    before, M, E = [], h.abs(), torch.zeros_like(h)
+    for t in range(T):
+        before.append((h, M, E))
+        h, M, E = token(p, t, h, M, E)
+        out, err = h, E
+        if width == 3 * dim:
+            _, _, zs = gate_of(p, t)
+            out, err = h * zs, (E + 2.0**-19 * h.abs()) * zs.abs()
+        y[:, t], ey[:, t] = torch.where(t < n, out, 0.0), torch.where(t < n, err, 0.0)
+    last = h, E
+    if keep == "int8":
+        for t in range(T):
+            if t % EVERY:
+                before[t] = token(q, t - 1, *before[t - 1])
+    dp, ep = torch.zeros(2, B, T, width, dtype=torch.float64)
+    c, Mc, Ec = dh, dh.abs(), torch.zeros_like(dh)
+    for t in range(T - 1, -1, -1):
+        if t + 1 == seam:
+            c = torch.zeros_like(c)
+        x, f, k = gates(q, t)
+        hp, Mp, Ep = before[t]
+        d, parts, errors = dy[:, t], [], []
+        up, eu = d, 0.0 * d
+        if width == 3 * dim:
+            z, s, zs = gate_of(q, t)
+            hn, _, En = token(q, t, hp, Mp, Ep)
+            slope = s + zs * (1 - s)
+            off = 2.0**-18 * (s + (zs * (1 - s)).abs()) + 2.0**-23 * zs.abs()
+            parts, errors = [d * hn * slope], [d.abs() * (En * slope.abs() + hn.abs() * off)]
+            up, eu = d * zs, 2.0**-19 * (d * zs).abs()
+        g, M, E = up + c, up.abs() + Mc, eu + Ec + U * (up.abs() + Mc)
+        least = GATE * torch.minimum(f, k)
+        errors = [
+            k * E + (least + U * k) * M,
+            k * f * (E * (hp - x).abs() + M * Ep + M * 2 * GATE * (hp - x).abs() + U * M * (hp.abs() + x.abs())),
+        ] + errors
+        parts = [g * k, g * (hp - x) * f * k] + parts
+        live = t < n
+        dp[:, t], ep[:, t] = torch.where(live, torch.cat(parts, -1), 0.0), torch.where(live, torch.cat(errors, -1), 0.0)
+        c, Mc, Ec = (torch.where(live, a, b) for a, b in ((g * f, c), (M * f, Mc), (f * E + (least + U * f) * M, Ec)))
+    return (y, ey), last, (dp, ep), (c, Ec)
+
+
+def outside(got, bound):
+    """How far beyond its bound and its rounding an element is, at most (0: none is)."""
+    want, error = bound
+    got = got.detach().cpu()
+    allowed = torch.finfo(got.dtype).eps / 2 * want.abs() + error
+    allowed = 1.01 * allowed + (2.0**-25 if got.dtype == torch.float16 else 1e-37)
+    assert got.isfinite().all()
+    return float(((got.double() - want).abs() - allowed).clamp_min(0).max()) if got.numel() else 0.0
+
+
+def check_bounds(p, D, h0, lengths, dy, dh, keep):
+    p, h = p.detach().requires_grad_(), h0.detach().requires_grad_()
+    y, last = gated_scan(p, D, h, lengths, keep=keep)
+    dp, dh0 = torch.autograd.grad((y, last), (p, h), (dy, dh))
+    for what, got, bound in zip(("y", "h_last", "dp", "dh0"), (y, last, dp, dh0), bounded(p, D, h0, lengths, dy, dh, keep)):
+        assert outside(got, bound) == 0, (what, outside(got, bound))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "plain"])
+@pytest.mark.parametrize("B,T,D", [(3, 1, 5), (3, 37, 33), (2, 150, 40)])
+def test_every_element_is_within_its_bound(device, dtype, keep, gate, B, T, D):
+    p, h0, dy, dh = inputs(B, T, D, dtype, device, gate)
+    lengths = torch.tensor([T, T // 2, 1][:B], device=device)
+    check_bounds(p, D, h0, lengths, dy, dh, keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize(
+    "B,T,D",
+    [
+        (1, 513, 64),    # chained blocks
+        (1, 2049, 40),
+        (2, 5000, 33),   # several links
+        (4, 2300, 200),  # links of 16 tiles
+        (5, 1100, 130),
+        (700, 150, 50),  # a block walks several tiles
+        (2200, 70, 62),  # a wave walks alone
+        (4100, 40, 25),  # staged
+        (2100, 40, 100),
+        (3, 4, 130),     # short tiles
+    ],
+)
+def test_every_element_of_every_layout(B, T, D, dtype, keep):
+    p, h0, dy, dh = inputs(B, T, D, dtype, "cuda")
+    lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(2)).cuda()
+    lengths[-1] = T
+    check_bounds(p, D, h0, lengths, dy, dh, keep)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", [(1, 513, 64), (2, 2500, 33)])
+def test_the_bounds_tell_mistakes(dtype, B, T, D):
+    """Planted in the oracle: a carry that is lost at one token, and results 1% too large."""
+    p, h0, dy, dh = inputs(B, T, D, dtype, "cpu")
+    right = bounded(p, D, h0, None, dy, dh)
+    assert all(outside(v.to(dtype if i in (0, 2) else torch.float32), right[i]) == 0 for i, (v, _) in enumerate(right))
+    lost = bounded(p, D, h0, None, dy, dh, seam=T // 2)
+    for part in range(3):
+        at = slice(part * D, (part + 1) * D)
+        v, e = right[2][0][..., at], right[2][1][..., at]
+        assert outside((v * 1.01).to(dtype), (v, e)) > 0
+        if part < 2:  # dz does not know the carry
+            assert outside(lost[2][0][..., at].to(dtype), (v, e)) > 0
+    assert outside((right[0][0] * 1.01).to(dtype), right[0]) > 0
+    assert outside((right[3][0] * 1.01).float(), right[3]) > 0
+    first = bounded(p, D, h0, None, dy, dh, seam=1)
+    assert outside(first[3][0].float(), right[3]) > 0
