@@ -45,7 +45,8 @@ def _lstm_layer(x, w_ih_t, w_hh_t, b, H, checkpoint8=False):
     then per step one mm + ATen's fused differentiable LSTM cell (the same
     pointwise kernel torch.nn.LSTM uses on CUDA; dispatching it directly
     bypasses the slow MIOpen RNN route on ROCm). With ``checkpoint8`` the
-    projection keeps x as 8-bit codes, a quarter of its bytes."""
+    projection keeps x as 8-bit codes, a quarter of its bytes; the states of
+    each step, which the recurrent products and the cells keep, stay as they are."""
     B, T, I = x.shape
     # [T,B,4H] so each timestep slice is contiguous for the fused cell
     if checkpoint8:
@@ -73,12 +74,14 @@ def _lstm_layer(x, w_ih_t, w_hh_t, b, H, checkpoint8=False):
     return torch.stack(outs, dim=1)
 
 
-def wide_forward(module, x, checkpoint8=False):
-    """Full stacked forward: windows [B,T,F] -> head output [B,F_out]."""
+def wide_forward(module, x, checkpoint8=False, windows_stay=False):
+    """Full stacked forward: windows [B,T,F] -> head output [B,F_out].
+    ``windows_stay``: the caller holds x through the backward pass, so codes of
+    it (``checkpoint8``) would only come on top; layers behind the first have theirs."""
     packed = _packed_weights(module, x.device, x.dtype)
     h = x
-    for (w_ih_t, w_hh_t, b), cell in zip(packed, module.cells):
-        h = _lstm_layer(h, w_ih_t, w_hh_t, b, cell.hidden_size, checkpoint8)
+    for i, ((w_ih_t, w_hh_t, b), cell) in enumerate(zip(packed, module.cells)):
+        h = _lstm_layer(h, w_ih_t, w_hh_t, b, cell.hidden_size, checkpoint8 and not (windows_stay and i == 0))
     last = h[:, -1, :]
     return module.head_act(module.head(last))
 
@@ -117,7 +120,7 @@ class WideLSTMTrainer:
         # fp32 throughout: the step is kernel-count-bound, not GEMM-bound,
         # and the fused ATen cell is fp32-first
         def fwd_loss(w, tgt):
-            return loss_fn(wide_forward(module, w, getattr(cfg, "checkpoint8", False)), tgt)
+            return loss_fn(wide_forward(module, w, getattr(cfg, "checkpoint8", False), windows_stay=True), tgt)
 
         # ---- hipGraph capture of the whole fwd+bwd (static shapes) --------
         graph = None

@@ -545,3 +545,31 @@ def test_weight_gradient_of_infinite_dy(device, dtype, N):
     w = torch.randn(20, 40, device=device).to(dtype)
     frozen = torch.autograd.grad(linear8(x, w, b), b, dy)[0]
     assert same(frozen.isfinite().float(), db.isfinite().float()) and (frozen[1] == inf).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_wide_lstm_makes_no_codes_of_windows_that_stay(device):
+    """A training loop holds its windows through the backward pass: codes beside them would
+    be bytes more, not fewer. The layers behind keep codes of what they read."""
+    from gordo_amd.model.factories.lstm_autoencoder import lstm_symmetric
+    from gordo_amd.ops.wide_lstm import wide_forward
+
+    module = lstm_symmetric(n_features=12, dims=[40, 36], lookback_window=9).to(device)
+    w = torch.randn(6, 9, 12, device=device)
+
+    def kept_by(**how):
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+            out = wide_forward(module, w, **how)
+        codes = sorted(t.numel() for t in kept if t.dtype == torch.int8)
+        stays = any(t.untyped_storage().data_ptr() == w.untyped_storage().data_ptr() for t in kept)
+        return out, codes, stays
+
+    out, codes, stays = kept_by(checkpoint8=True, windows_stay=True)
+    full, none, _ = kept_by()
+    rows = 6 * 9
+    assert codes == sorted(rows * n for n in (64, 64, 64)) and stays and not none  # 40, 36 and 36 wide, padded to 64
+    assert torch.allclose(out, full, atol=1e-5)
+    assert kept_by(checkpoint8=True)[1] == sorted(rows * n for n in (32, 64, 64, 64))
+    first = [p for p in module.cells[-1].parameters()]
+    assert all(g.isfinite().all() for g in torch.autograd.grad(out.square().mean(), first))
