@@ -93,6 +93,7 @@ class WideLSTMTrainer:
         self.module = module
         self.device = device
         self.cfg = cfg
+        self.uses_checkpoint8 = len(module.cells) > 1  # the first layer's windows stay anyway
 
     def fit(self, X: np.ndarray, y: np.ndarray, lookback: int = 144, lookahead: int = 0) -> TrainHistory:
         cfg = self.cfg

@@ -111,13 +111,23 @@ class Trainer:
 
             engine = fused.maybe_fused_trainer(module, self.device, cfg)
             if engine is not None:
+                if not getattr(engine, "uses_checkpoint8", False):
+                    self._warn_checkpoint8(type(engine).__name__)
                 return engine.fit(X, y, lookback=lookback, lookahead=lookahead)
             logger.info(
                 "Fused engine unavailable for %s; using eager torch path",
                 type(module).__name__,
             )
 
+        self._warn_checkpoint8("the eager path")
         return self._fit_eager(module, X, y, lookback, lookahead)
+
+    def _warn_checkpoint8(self, engine: str) -> None:
+        if self.config.checkpoint8:
+            logger.warning(
+                "checkpoint8 has no effect on %s: it is for LSTM layers on the GPU "
+                "that are wider than the fused cells", engine,
+            )
 
     # ------------------------------------------------------------------
     def _fit_eager(

@@ -573,3 +573,43 @@ def test_wide_lstm_makes_no_codes_of_windows_that_stay(device):
     assert kept_by(checkpoint8=True)[1] == sorted(rows * n for n in (32, 64, 64, 64))
     first = [p for p in module.cells[-1].parameters()]
     assert all(g.isfinite().all() for g in torch.autograd.grad(out.square().mean(), first))
+
+
+def test_checkpoint8_without_effect_is_said(caplog):
+    """On estimators that have no such layers, and on the CPU, the argument changes nothing."""
+    import logging
+
+    import numpy as np
+
+    from gordo_amd.model.models import TorchAutoEncoder, TorchLSTMAutoEncoder
+
+    X = np.random.default_rng(0).normal(size=(40, 4)).astype(np.float32)
+    dense = dict(kind="feedforward_symmetric", dims=[4], funcs=["tanh"], epochs=1, device="cpu")
+    lstm = dict(kind="lstm_symmetric", dims=[4], funcs=["tanh"], lookback_window=3, epochs=1, device="cpu")
+    for model, args in ((TorchAutoEncoder, dense), (TorchLSTMAutoEncoder, lstm)):
+        with caplog.at_level(logging.WARNING):
+            model(**args).fit(X)
+            assert "checkpoint8" not in caplog.text
+            model(**args, checkpoint8=True).fit(X)
+            assert "checkpoint8 has no effect" in caplog.text
+        caplog.clear()
+
+
+@pytest.mark.gpu
+def test_checkpoint8_without_effect_is_said_of_fused_engines(caplog):
+    import logging
+
+    import numpy as np
+
+    from gordo_amd.model.models import TorchAutoEncoder, TorchLSTMAutoEncoder
+
+    X = np.random.default_rng(0).normal(size=(300, 10)).astype(np.float32)
+    with caplog.at_level(logging.WARNING):
+        TorchAutoEncoder(kind="feedforward_hourglass", epochs=1, checkpoint8=True).fit(X)
+        assert "checkpoint8 has no effect" in caplog.text
+        caplog.clear()
+        TorchLSTMAutoEncoder(kind="lstm_symmetric", dims=[16], lookback_window=6, epochs=1, batch_size=16, checkpoint8=True).fit(X)
+        assert "checkpoint8 has no effect" in caplog.text
+        caplog.clear()
+        TorchLSTMAutoEncoder(kind="lstm_symmetric", dims=[260], lookback_window=6, epochs=1, batch_size=16, checkpoint8=True).fit(X[:40])
+        assert "checkpoint8" not in caplog.text
