@@ -471,7 +471,7 @@ unsigned int c8_blocks(int64_t lanes) {
 
 unsigned int c8_works(int64_t eights) {
     const int64_t n = (eights + 256 * C8_WORK - 1) / (256 * C8_WORK);
-    TORCH_CHECK(n <= INT_MAX, "checkpoint8: too many values");
+    TORCH_CHECK(n * 256 <= UINT32_MAX, "checkpoint8: too many values");  // a launch takes fewer than 2^32 threads
     return (unsigned int)n;
 }
 
@@ -597,7 +597,7 @@ void weight_grad8_launch(torch::Tensor dy, torch::Tensor codes, torch::Tensor sc
     const int64_t tiles = (int64_t)a.tiles_f * a.tiles_o, Fq = (F + 3) / 4 * 4, Oq = (O + 3) / 4 * 4;
     a.per = plan.steps * WG_K;
     a.splits = plan.splits;
-    TORCH_CHECK(tiles * a.splits <= INT_MAX, "weight_grad8: sizes out of range");
+    TORCH_CHECK(tiles * a.splits * WG_THREADS <= UINT32_MAX, "weight_grad8: sizes out of range");
     // whole 16-byte words, and a tile's rows within 31-bit offsets
     const bool aligned = O % 8 == 0 && a.sdy % 8 == 0 && a.sdy >= O && a.sdy <= (1 << 22) && (uintptr_t)a.dy % 16 == 0;
     torch::Tensor part, part_b;

@@ -981,6 +981,12 @@ struct GsPlan {
     size_t lds;
 };
 
+// A launch takes fewer than 2^32 threads.
+unsigned int gs_blocks(int64_t blocks, int threads, const char* what) {
+    TORCH_CHECK(blocks * threads <= UINT32_MAX, what, ": sizes of p out of range");
+    return (unsigned int)blocks;
+}
+
 GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hipStream_t stream) {
     GsPlan plan{};
     const int64_t groups = ((int64_t)a.B * a.tps + 63) / 64;
@@ -999,16 +1005,17 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
         a.pitch_p = (plan.R * parts * a.D * es + 7) / 4 * 4;
         a.pitch_y = (plan.R * a.D * es + 7) / 4 * 4;
         a.nJ = (a.T + plan.R - 1) / plan.R;
-        plan.blocks = (unsigned int)((a.B + a.seqs - 1) / a.seqs);
+        plan.blocks = gs_blocks(((int64_t)a.B + a.seqs - 1) / a.seqs, 64, "gated_scan");
         const int p_in = a.dy != nullptr && a.codes != nullptr ? 0 : a.pitch_p;
         plan.lds = (size_t)a.seqs * (p_in + a.pitch_y + (a.dy != nullptr ? a.pitch_p : 0));
         return plan;
     }
     a.groups = (int)groups;
     a.nJ = (a.T + plan.W * plan.R - 1) / (plan.W * plan.R);
-    int64_t blocks = groups;
-    if (plan.W > 1 && groups < 512 && a.nJ > 4) {
-        blocks = groups * a.nJ;
+    const bool chained = plan.W > 1 && groups < 512 && a.nJ > 4;
+    const int64_t blocks = chained ? groups * a.nJ : groups;
+    plan.blocks = gs_blocks(blocks, 64 * plan.W, "gated_scan");
+    if (chained) {
         // Links of 16 tiles, where those take as long as a link by their bytes; else 32
         // (1 sequence of 131072 tokens, 64 channels: 58 + 111 us in links of 16, 45 + 76 of 32).
         a.lb = groups * plan.W * V < 32 ? GS_LB : 16;
@@ -1021,8 +1028,6 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
         a.prefix = (unsigned int*)(at + 16 + words * 8);
         hipLaunchKernelGGL(gs_clear, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, stream, (uint4*)at, n);
     }
-    TORCH_CHECK(blocks <= INT_MAX, "gated_scan: too many blocks");
-    plan.blocks = (unsigned int)blocks;
     return plan;
 }
 
@@ -1090,7 +1095,7 @@ struct GsStepCall {
     hipStream_t stream;
     template <class E, int V, int P>
     void operator()() {
-        hipLaunchKernelGGL((gs_step<E, V, P>), dim3(a.B), dim3(threads), 0, stream, a);
+        hipLaunchKernelGGL((gs_step<E, V, P>), dim3(gs_blocks(a.B, threads, "gated_step")), dim3(threads), 0, stream, a);
     }
 };
 

@@ -963,3 +963,15 @@ def test_the_bounds_tell_mistakes(dtype, B, T, D):
     assert outside((right[3][0] * 1.01).float(), right[3]) > 0
     first = bounded(p, D, h0, None, dy, dh, seam=1)
     assert outside(first[3][0].float(), right[3]) > 0
+
+
+@pytest.mark.gpu
+def test_more_than_a_launch_takes_is_refused():
+    """2^32 threads and more: said before anything is launched."""
+    row = torch.zeros(2, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="out of range"):
+        gated_scan(row.expand(1, 2**30, 2), 1)
+    with pytest.raises(RuntimeError, match="out of range"):
+        gated_step(row.expand(2**26, 2), torch.zeros(2**26, 1, device="cuda"))
+    y = gated_step(row.expand(2**20, 2), torch.ones(2**20, 1, device="cuda"))
+    assert (y == 0.5).all()
