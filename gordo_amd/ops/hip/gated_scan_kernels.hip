@@ -538,6 +538,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
         // h_last comes from the wave that has the last token: what is behind it in its tile
         // is padding, which passes the state on
         const bool last = l.live && tile == max(l.len - 1, 0) / R;
+        const int rows = l.live ? l.len - t0 : 0;  // tokens of the tile that are there, if more than 0
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float out[V];
@@ -552,15 +553,17 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
                 }
             }
             if constexpr (STAGE) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) out[v] = t0 + i >= l.len ? 0.f : out[v];
                 if (l.live) pack::put((typename E::store*)(mine_y + i * a.D * ES), out);
-            } else if (l.live && t0 + i < l.len) {
+            } else if (i < rows) {
                 pack::put(y + (int64_t)(t0 + i) * a.D, out);
             }
             gs_fence<W>(i);
         }
         if constexpr (STAGE) {
+            if (!whole && l.live) {
+                const float zero[V] = {};
+                for (int i = max(rows, 0); i < R; ++i) pack::put((typename E::store*)(mine_y + i * a.D * ES), zero);
+            }
             gs_taken();
             for (int s = 0; s < a.seqs; ++s) {
                 const int64_t b = cg * (int64_t)a.seqs + s;
@@ -735,6 +738,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
         // a time: the first half's are computed twice. A wave alone keeps all of them (8192
         // sequences of 144 tokens, 70 channels: 356 us, in halves 384; 25 channels as codes,
         // where all of them cost a wave a SIMD: 142, in halves 112).
+        const int rows = l.live ? l.len - t0 : 0;  // tokens of the tile that are there, if more than 0
         constexpr int SPAN = W == 1 && !KEEP ? R : R / 2;
         float first[V], before[SPAN][V];
 #pragma unroll
@@ -783,13 +787,11 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
                     out[1][v] = fmaf(small, hp, -(small * x)) * more;  // small is at most 1/2: the difference does not overflow
                 }
                 if constexpr (STAGE) {
+                    if (l.live) {
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) out[q][v] = t0 + i >= l.len ? 0.f : out[q][v];
-                        if (l.live) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), out[q]);
+                        for (int q = 0; q < P; ++q) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), out[q]);
                     }
-                } else if (l.live && t0 + i < l.len) {
+                } else if (i < rows) {
 #pragma unroll
                     for (int q = 0; q < P; ++q) pack::put(dp + ((int64_t)(t0 + i) * P + q) * a.D, out[q]);
                 }
@@ -799,6 +801,12 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
             for (int v = 0; v < V; ++v) h[v] = first[v];
         }
         if constexpr (STAGE) {
+            if (!whole && l.live) {
+                const float zero[V] = {};
+                for (int i = max(rows, 0); i < R; ++i)
+#pragma unroll
+                    for (int q = 0; q < P; ++q) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), zero);
+            }
             gs_taken();
             for (int s = 0; s < a.seqs; ++s) {
                 const int64_t b = cg * (int64_t)a.seqs + s;
