@@ -7,7 +7,8 @@ need a scale, one for each 32 values of a row:
 
     e     = max(floor(log2 max|v|) - 6, -126)         kept as the byte e + 127
     code  = clamp(rint(v / 2^e), -127, 127)           int8
-    value = code * 2^e                                |value - v| <= max|v| / 127
+    value = code * 2^e                                |value - v| <= max|v| / 127,
+                                                      or 2^-127 where that is more
 
 The scale is a power of two, so a kept value has at most seven significant bits
 and is exact in bf16 and fp16: products take it as it is. A group with a value
@@ -81,7 +82,8 @@ def values_eager(codes: torch.Tensor, scales: torch.Tensor, F: int) -> torch.Ten
 
 
 def save8(x: torch.Tensor) -> Saved8:
-    """The 8-bit codes of ``x``, groups of 32 along its last axis."""
+    """The 8-bit codes of ``x``, groups of 32 along its last axis. Codes carry no
+    gradient: this is what a backward pass keeps, not a layer."""
     rows = _rows(x, "x")
     if rows.is_cuda:
         codes, scales = ext().save8(rows)

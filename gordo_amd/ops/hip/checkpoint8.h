@@ -6,7 +6,8 @@
 // costs up to one of the eight bits against max|v|/127, and buys exactness:
 // v / 2^e and code * 2^e are exact in 32 bits, and code * 2^e has at most seven
 // significant bits, so it is exact in bf16 and fp16 too and goes into a matrix
-// product without a rounding of its own. |code * 2^e - v| <= max|v| / 127.
+// product without a rounding of its own. |code * 2^e - v| <= max|v| / 127, or 2^-127
+// where that is more (groups below 2^-120, whose e has no further to go).
 // Byte 255: a value of the group was not finite; the whole group restores as NaN.
 #pragma once
 #include <hip/hip_runtime.h>

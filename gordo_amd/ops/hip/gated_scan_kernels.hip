@@ -562,7 +562,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 2 : W == 4 ? 3 : 4) void gs_fwd(Gs
         if constexpr (STAGE) {
             if (!whole && l.live) {
                 const float zero[V] = {};
-                for (int i = max(rows, 0); i < R; ++i) pack::put((typename E::store*)(mine_y + i * a.D * ES), zero);
+                for (int i = max(rows, 0); i < min(R, a.T - t0); ++i) pack::put((typename E::store*)(mine_y + i * a.D * ES), zero);
             }
             gs_taken();
             for (int s = 0; s < a.seqs; ++s) {
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
         // Beside other waves, and where codes take registers too, the states of half a tile at
         // a time: the first half's are computed twice. A wave alone keeps all of them (8192
         // sequences of 144 tokens, 70 channels: 356 us, in halves 384; 25 channels as codes,
-        // where all of them cost a wave a SIMD: 142, in halves 112).
+        // where they would cost a wave a SIMD: 142, in halves 112).
         const int rows = l.live ? l.len - t0 : 0;  // tokens of the tile that are there, if more than 0
         constexpr int SPAN = W == 1 && !KEEP ? R : R / 2;
         float first[V], before[SPAN][V];
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
         if constexpr (STAGE) {
             if (!whole && l.live) {
                 const float zero[V] = {};
-                for (int i = max(rows, 0); i < R; ++i)
+                for (int i = max(rows, 0); i < min(R, a.T - t0); ++i)
 #pragma unroll
                     for (int q = 0; q < P; ++q) pack::put((typename E::store*)(mine_dp + (i * P + q) * a.D * ES), zero);
             }
@@ -971,16 +971,18 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
 // fits 128 registers a lane: blocks of 8 waves, 4 waves a SIMD. The codes and the
 // backward pass need up to 168: blocks of 4, 3 waves a SIMD.
 // Staging: where a wave walks alone, narrow rows that are not whole sectors (64 bytes) go
-// through LDS: 8192 sequences of 144 tokens, 25 channels in bf16, take 53 + 75 us that way,
-// forward and backward, and 64 + 102 row by row. Rows of up to 64 channels have a lane for
-// each: more waves, more loads under way (144 tokens, 50 channels, x | r | z: 115 + 220 us,
-// 147 + 283 in pairs). In tiles of 4 tokens a wave has little to do, and pairs, which give
-// it two rows, are faster (200000 of 3 tokens, 50 channels: 85 + 133, and 115 + 154 a lane
-// each). Rows of 66 to 128 channels go in pairs (8192 x 144 x 70: 161 + 346, row by row 196
-// + 385), but not into codes (16384 x 40 x 100: 227 + 230, row by row 188 + 167) and not
-// in tiles of 4 (200000 x 3 x 100: 145 + 245, row by row 141 + 248).
+// through LDS: 8192 sequences of 144 tokens, 25 channels in bf16, take 49 + 78 us that way,
+// forward and backward, and 50 + 108 row by row. Rows of up to 64 channels have a lane for
+// each: more waves, more loads under way (144 tokens, 50 channels, x | r | z: 119 + 210 us,
+// 151 + 292 in pairs). In tiles of 4 tokens a wave has little to do, and pairs, which give
+// it two rows, are faster (200000 of 3 tokens, 50 channels: 91 + 133, and 126 + 162 a lane
+// each). Rows of 66 to 128 channels go in pairs (8192 x 144 x 70: 163 + 349, row by row 191
+// + 384), but not into codes (16384 x 40 x 100: 234 + 250, row by row 192 + 185), not in
+// tiles of 4 (200000 x 3 x 100: 154 + 238, row by row 142 + 251), and not where an eighth
+// and more of the tiles' tokens do not exist: LDS has room for two waves a SIMD, which
+// walk them all the same (30000 x 40 x 70: 189 + 415, row by row 190 + 358).
 // Sequences of up to 4 tokens have tiles of 4 (32768 of one token, 1024 channels:
-// forward 221 us in tiles of 16, 113 in tiles of 4).
+// forward 284 us in tiles of 16, 117 in tiles of 4).
 struct GsPlan {
     int W, R;
     unsigned int blocks;
@@ -1005,7 +1007,8 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
     const int es = (int)p.element_size();
     const bool narrow = a.D <= 64, brief = plan.R < GS_R;
     const int stage = V == 2 && narrow == brief ? 2 : 1;
-    const bool fits = narrow || (a.D <= 128 && stage == 2 && a.codes == nullptr);
+    const bool full = ((int64_t)a.T + plan.R - 1) / plan.R * plan.R * 8 <= (int64_t)a.T * 9;
+    const bool fits = narrow || (a.D <= 128 && stage == 2 && a.codes == nullptr && full);
     if (plan.W == 1 && fits && a.D * es % 64 != 0 && (a.T == 1 || (a.st == (int64_t)parts * a.D && (a.dy == nullptr || a.dst == a.D)))) {
         plan.staged = stage;
         a.tps = (a.codes != nullptr ? a.Dp : a.D) / stage;
@@ -1025,7 +1028,8 @@ GsPlan gs_plan(GsArgs& a, int V, int many, int parts, const torch::Tensor& p, hi
     plan.blocks = gs_blocks(blocks, 64 * plan.W, "gated_scan");
     if (chained) {
         // Links of 16 tiles, where those take as long as a link by their bytes; else 32
-        // (1 sequence of 131072 tokens, 64 channels: 58 + 111 us in links of 16, 45 + 76 of 32).
+        // (1 sequence of 131072 tokens, 64 channels: 61 + 108 us in links of 16, 47 + 75 of 32;
+        // of 65536 tokens, 768 channels: 106 + 174 of 16, 108 + 198 of 32).
         a.lb = groups * plan.W * V < 32 ? GS_LB : 16;
         const int64_t words = blocks * V * 64, links = (int64_t)((a.nJ + a.lb - 1) / a.lb) * groups * V * 64;
         const int64_t n = (words * 8 + links * 4 + 16 + 15) / 16;
