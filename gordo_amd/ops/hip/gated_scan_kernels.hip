@@ -168,8 +168,8 @@ __device__ __forceinline__ GsLane gs_lane_staged(const GsArgs& a, int64_t cg, in
 
 // ---------------------------------------------------------------------------
 // Staging of narrow rows. Rows of 25 or 50 channels start and end inside a memory
-// sector; written row by row, every sector is written in pieces (2.8 TB/s at 25
-// channels against 5.3 at 32). But a sequence's tile of GS_R rows is one run of bytes:
+// sector; written row by row, every sector is written in pieces (backward 2.8 TB/s at 25
+// channels against 4.6 at 32). But a sequence's tile of GS_R rows is one run of bytes:
 // it goes through LDS, and memory sees whole words of the run, 256 bytes at a time.
 // A run starts at any 2-byte address; in LDS it keeps its place within a word, so a
 // word of memory is a word of LDS. A load may take the other half of the run's first
