@@ -1,14 +1,14 @@
 // Gated linear recurrence over a batch of sequences, its gradient, and its
 // one-token form.
 //
-//   p = [x | r | z] along the last axis (z optional), k = sigmoid(-r)
-//   h_t = h_{t-1} + k_t (x_t - h_{t-1})        ( = (1-k) h + k x )
+//   p = [x | r | z] along the last axis (z optional), f = sigmoid(r), k = 1 - f
+//   h_t = f_t h_{t-1} + k_t x_t
 //   y_t = h_t * z_t * sigmoid(z_t)             (y_t = h_t without z)
 //
 // A long memory has k near 0, where 1 - k in 32 bits has lost k's digits; a token that
 // lets the state go has f = 1 - k near 0, where k has lost f's. So a gate is kept as the
-// smaller of the two, and which it is (gs_gate). Every state is held in 32 bits; only y and dp are
-// rounded, once, to the type of p.
+// smaller of the two, and which it is (gs_gate). Every state is held in 32 bits; only y
+// and dp are rounded, once, to the type of p.
 //
 // A wave owns 64 * V channels (V neighbours a lane) and takes GS_R tokens at a
 // time: all their loads are issued before the first is used, so that enough
@@ -738,8 +738,8 @@ __global__ __launch_bounds__(64 * W, W == 1 ? (V == 1 && sizeof(typename E::stor
         // a time: the first half's are computed twice. A wave alone keeps all of them (8192
         // sequences of 144 tokens, 70 channels: 356 us, in halves 384; 25 channels as codes,
         // where they would cost a wave a SIMD: 142, in halves 112).
-        const int rows = l.live ? l.len - t0 : 0;  // tokens of the tile that are there, if more than 0
         constexpr int SPAN = W == 1 && !KEEP ? R : R / 2;
+        const int rows = l.live ? l.len - t0 : 0;  // tokens of the tile that are there, if more than 0
         float first[V], before[SPAN][V];
 #pragma unroll
         for (int v = 0; v < V; ++v) first[v] = h[v];
@@ -978,8 +978,8 @@ void gs_f32(const torch::Tensor& t, int64_t n, const torch::Tensor& p, const cha
 // it two rows, are faster (200000 of 3 tokens, 50 channels: 91 + 133, and 126 + 162 a lane
 // each). Rows of 66 to 128 channels go in pairs (8192 x 144 x 70: 163 + 349, row by row 191
 // + 384), but not into codes (16384 x 40 x 100: 234 + 250, row by row 192 + 185), not in
-// tiles of 4 (200000 x 3 x 100: 154 + 238, row by row 142 + 251), and not where an eighth
-// and more of the tiles' tokens do not exist: LDS has room for two waves a SIMD, which
+// tiles of 4 (200000 x 3 x 100: 154 + 238, row by row 142 + 251), and not where tiles
+// have over an eighth more tokens than there are: LDS has room for two waves a SIMD, which
 // walk them all the same (30000 x 40 x 70: 189 + 415, row by row 190 + 358).
 // Sequences of up to 4 tokens have tiles of 4 (32768 of one token, 1024 channels:
 // forward 284 us in tiles of 16, 117 in tiles of 4).

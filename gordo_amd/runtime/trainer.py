@@ -53,8 +53,8 @@ class TrainConfig:
     verbose: int = 0
     seed: Optional[int] = None
     use_graph: bool = True  # hipGraph-capture the fused train step
-    # LSTM layers wider than the fused cells keep their inputs as 8-bit codes
-    # for the backward pass (ops.linear8)
+    # LSTM layers wider than the fused cells, behind the first, keep their inputs
+    # as 8-bit codes for the backward pass (ops.linear8)
     checkpoint8: bool = False
 
     @classmethod
