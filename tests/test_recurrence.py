@@ -975,3 +975,18 @@ def test_more_than_a_launch_takes_is_refused():
         gated_step(row.expand(2**26, 2), torch.zeros(2**26, 1, device="cuda"))
     y = gated_step(row.expand(2**20, 2), torch.ones(2**20, 1, device="cuda"))
     assert (y == 0.5).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("keep", ["input", "int8"])
+@pytest.mark.parametrize("B,T,D", [(3, 4, 20), (2, 90, 33), (2, 100, 130), (1, 1300, 64)])
+def test_every_element_with_gates_of_every_size(device, dtype, keep, B, T, D):
+    """Tokens that let all of the state go among ones that hold all of it."""
+    p, h0, dy, dh = inputs(B, T, D, dtype, "cpu")
+    r = (torch.randn(B, T, D, generator=torch.Generator().manual_seed(6)) * 6).clamp(-15.9, 15.9)
+    p[..., D : 2 * D] = r.to(dtype)
+    lengths = torch.full((B,), T)
+    lengths[0] = T - 1
+    p, h0, lengths, dy, dh = (t.to(device) for t in (p, h0, lengths, dy, dh))
+    check_bounds(p, D, h0, lengths, dy, dh, keep)
